@@ -1,4 +1,5 @@
-"""Builds ``libelx_hip.so`` in-tree with hipcc for gfx950.
+"""Builds ``libelx_hip.so`` (the optimizer step) and ``libelx_ops.so`` (the operators beside it) in-tree with hipcc for
+gfx950.
 
     python -m elixir_amd.build
 
@@ -11,6 +12,7 @@ import shutil
 import subprocess
 import sys
 
+from . import _ops_abi
 from ._abi import LIB_PATH, built_source_sha, source_sha16
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -18,6 +20,8 @@ _ROOT = os.path.dirname(_HERE)
 SOURCES = [os.path.join(_HERE, 'csrc', 'elx_kernels.hip'), os.path.join(_HERE, 'csrc', 'elx_host.cpp')]
 HOST_SOURCE = os.path.join(_HERE, 'csrc', 'elx_host.cpp')
 OUTPUT = LIB_PATH
+OPS_SOURCES = [f for f in _ops_abi.source_files() if f.endswith(('.hip', '.cpp'))]
+OPS_OUTPUT = _ops_abi.LIB_PATH
 
 HIPCC_FLAGS = [
     '--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-shared', '-ffp-contract=off', '-Xclang', '-target-feature',
@@ -33,17 +37,25 @@ def hipcc_path() -> str:
 
 
 def build(verbose: bool = True) -> str:
-    cmd = ([hipcc_path()] + HIPCC_FLAGS + [f'-DELX_SOURCE_SHA="{source_sha16()}"', '-I', os.path.join(_ROOT, 'include'),
-                                           '-o', OUTPUT] + SOURCES)
-    if verbose:
-        print(' '.join(cmd), flush=True)
-    proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    # the host pass does not know the device-only target feature and says so; that is harmless
-    out = '\n'.join(l for l in proc.stdout.splitlines() if 'packed-fp32-ops' not in l)
-    if proc.returncode != 0:
-        raise RuntimeError(f'hipcc failed ({proc.returncode}):\n{out}')
-    if verbose and out.strip():
-        print(out)
+    """Compiles both libraries, side by side; returns the path of ``libelx_hip.so``."""
+    head, include = [hipcc_path()] + HIPCC_FLAGS, ['-I', os.path.join(_ROOT, 'include')]
+    cmds = [head + [f'-DELX_SOURCE_SHA="{source_sha16()}"'] + include + ['-o', OUTPUT] + SOURCES,
+            head + [f'-DELX_OPS_SOURCE_SHA="{_ops_abi.source_sha16()}"'] + include + ['-o', OPS_OUTPUT] + OPS_SOURCES]
+    procs = []
+    for cmd in cmds:
+        if verbose:
+            print(' '.join(cmd), flush=True)
+        procs.append(subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))
+    failed = []
+    for proc in procs:
+        # the host pass does not know the device-only target feature and says so; that is harmless
+        out = '\n'.join(l for l in proc.communicate()[0].splitlines() if 'packed-fp32-ops' not in l)
+        if proc.returncode != 0:
+            failed.append(f'hipcc failed ({proc.returncode}):\n{out}')
+        elif verbose and out.strip():
+            print(out)
+    if failed:
+        raise RuntimeError('\n'.join(failed))
     return OUTPUT
 
 
@@ -61,8 +73,9 @@ def build_host_checked(out_path: str, verbose: bool = False) -> str:
 
 
 def is_stale() -> bool:
-    """The built library is missing, or was built from other sources than the ones beside it."""
-    return not os.path.exists(OUTPUT) or built_source_sha(OUTPUT) != source_sha16()
+    """A built library is missing, or was built from other sources than the ones beside it."""
+    return (not os.path.exists(OUTPUT) or built_source_sha(OUTPUT) != source_sha16() or not os.path.exists(OPS_OUTPUT)
+            or _ops_abi.built_source_sha(OPS_OUTPUT) != _ops_abi.source_sha16())
 
 
 def ensure_built(verbose: bool = False) -> str:

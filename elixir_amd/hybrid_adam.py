@@ -10,6 +10,9 @@ Two ways in:
   exp_avg_sq are flat fp32 buffers per chunk, gradients are read from the low-precision shards and
   the refreshed low-precision parameters are written back by the same launch.
 
+With ``state_bits=8`` both moments are held in 8 bits: 2 bytes per element and 2 more per block of 256 instead of
+8, and a step moves 16 bytes per element instead of 28 (``include/elx_ops.h`` has the code and its rounding).
+
 Either way one step is one launch over every tensor of every parameter group.  The arithmetic
 follows ``torch.optim.Adam`` / ``AdamW`` (float64 host scalars narrowed to fp32, same op order);
 there is no CPU path.  "Hybrid" in the reference means GPU kernels for device-resident shards and
@@ -23,15 +26,16 @@ import numpy as np
 import torch
 from torch.optim import optimizer as _torch_optimizer
 
-from . import _abi
+from . import _abi, _ops_abi
 from .chunk import gpu_device, Chunk, DeviceTable, dtype_code
 from .launch_plan import FlatBuffer, LaunchPlan, build_plan
 
 
 def make_hyper_record(lr: float, beta1: float, beta2: float, eps: float, weight_decay: float, step: int,
-                      bias_correction: bool, adamw_mode: bool) -> np.ndarray:
+                      bias_correction: bool, adamw_mode: bool, state_bits: int = 32) -> np.ndarray:
     """Host scalars of one (group, step) pair -- torch/optim/adam.py:414-430,528-535 -- narrowed
-    to fp32 where a tensor op would narrow a Python scalar."""
+    to fp32 where a tensor op would narrow a Python scalar.  For an 8-bit state the step count rides in
+    the upper bits of the flags: the rounding of exp_avg_sq depends on it."""
     rec = np.zeros(1, dtype=_abi.HYPER_DTYPE)
     bc1 = 1.0 - beta1**step if bias_correction else 1.0
     bc2 = 1.0 - beta2**step if bias_correction else 1.0
@@ -57,23 +61,24 @@ def make_hyper_record(lr: float, beta1: float, beta2: float, eps: float, weight_
     rec['bc2_sqrt'] = math.sqrt(bc2)
     rec['eps'] = eps
     rec['neg_step'] = -(lr / bc1)
-    rec['flags'] = flags
+    rec['flags'] = flags | (step & 0xFFFFFF) << 8 if state_bits == 8 else flags
     return rec
 
 
 _HYPER_RECORDS: Dict = {}
 
 
-def hyper_record_cached(key: Tuple, adamw_mode: bool) -> np.ndarray:
+def hyper_record_cached(key: Tuple, adamw_mode: bool, state_bits: int = 32) -> np.ndarray:
     """``make_hyper_record`` for ``key = (lr, beta1, beta2, eps, weight_decay, step, bias_correction)``, kept:
     a step looks up the records the step before it has already computed while its launch was running."""
-    rec = _HYPER_RECORDS.get((key, adamw_mode))
+    rec = _HYPER_RECORDS.get((key, adamw_mode, state_bits))
     if rec is None:
         if len(_HYPER_RECORDS) > 4096:
             _HYPER_RECORDS.clear()
             _HYPER_ADDRESSES.clear()
         lr, b1, b2, eps, wd, step, bc = key
-        rec = _HYPER_RECORDS[(key, adamw_mode)] = make_hyper_record(lr, b1, b2, eps, wd, step, bc, adamw_mode)
+        rec = make_hyper_record(lr, b1, b2, eps, wd, step, bc, adamw_mode, state_bits)
+        _HYPER_RECORDS[(key, adamw_mode, state_bits)] = rec
         rec.flags.writeable = False    # shared between steps: nobody edits it
     return rec
 
@@ -81,13 +86,13 @@ def hyper_record_cached(key: Tuple, adamw_mode: bool) -> np.ndarray:
 _HYPER_ADDRESSES: Dict = {}
 
 
-def hyper_record_address(key: Tuple, adamw_mode: bool) -> int:
+def hyper_record_address(key: Tuple, adamw_mode: bool, state_bits: int = 32) -> int:
     """Host address of the cached record for ``key`` (the record stays alive in the cache, which is emptied
     together with this table)."""
-    ptr = _HYPER_ADDRESSES.get((key, adamw_mode))
+    ptr = _HYPER_ADDRESSES.get((key, adamw_mode, state_bits))
     if ptr is None:
-        rec = hyper_record_cached(key, adamw_mode)    # may empty both tables first
-        ptr = _HYPER_ADDRESSES[(key, adamw_mode)] = rec.ctypes.data
+        rec = hyper_record_cached(key, adamw_mode, state_bits)    # may empty both tables first
+        ptr = _HYPER_ADDRESSES[(key, adamw_mode, state_bits)] = rec.ctypes.data
     return ptr
 
 
@@ -115,8 +120,12 @@ class _SteadyStep:
         self.watch, self.layout, self.states, self.step = watch, layout, prep.states, step
         self.group_of_hyper = group_of_hyper      # group index of every hyper record, in table order
         self.dplan, self.grad_code, self.device = prep.dplan, prep.grad_code, prep.device
-        self.call = _abi.load().elx_adam_step_put_mt
-        self.fixed = (prep.dplan.rows.ptr, len(plan.rows), prep.dplan.segs.ptr, len(plan.segs))
+        if plan.state_rows is not None:
+            self.call = _ops_abi.load().elx_adam8_step_args_mt
+            self.fixed = (prep.dplan.rows.ptr, prep.dplan.state.ptr, len(plan.rows), prep.dplan.segs.ptr, len(plan.segs))
+        else:
+            self.call = _abi.load().elx_adam_step_put_mt
+            self.fixed = (prep.dplan.rows.ptr, len(plan.rows), prep.dplan.segs.ptr, len(plan.segs))
         self.tail = (plan.info.total_tiles, plan.info.max_tiles)
         self.flags = plan.info.flags
         n = len(group_of_hyper)
@@ -176,6 +185,8 @@ class _DevicePlan:
         self._gated_rows: Optional[DeviceTable] = None
         self.armed: Optional[torch.Tensor] = None    # one device word: whether the gated copy holds zeros right now
         self.segs = DeviceTable(plan.segs, device) if len(plan.segs) else None
+        # the rows of the 8-bit state, beside the update rows
+        self.state = DeviceTable(plan.state_rows, device) if plan.state_rows is not None and len(plan.rows) else None
         self.refresh = DeviceTable(plan.refresh_rows, device) if plan.refresh_rows is not None else None
         self.refresh_aligned = True
         if plan.refresh_rows is not None:
@@ -198,13 +209,15 @@ class ChunkBinding:
     """Where the fake parameters of ``ElixirOptimizer`` live: for each optimizer chunk the paired
     low-precision chunk, the flat m / v buffers and the slices the optimizer owns."""
 
-    def __init__(self, ranges: Dict[torch.nn.Parameter, Tuple[Chunk, int, int]]):
+    def __init__(self, ranges: Dict[torch.nn.Parameter, Tuple[Chunk, int, int]], state_bits: int = 32):
+        self.state_bits = state_bits
         # optimizer chunk -> index in the launch
         self.chunks: List[Chunk] = sorted({c for c, _, _ in ranges.values()})
         self.chunk_index = {c: i for i, c in enumerate(self.chunks)}
         self.ranges = ranges
         self.flat_m: Dict[Chunk, torch.Tensor] = {}
         self.flat_v: Dict[Chunk, torch.Tensor] = {}
+        self.flat_scales: Dict[Chunk, torch.Tensor] = {}    # 8-bit state: [blocks, 2] exponents of (exp_avg, exp_avg_sq)
         self.zero_grads = False        # the allocation step: gradients are zero, nothing is written back
         self.fused_writeback = False   # set by step(): the launch refreshed the low-precision shards
         for c in self.chunks:
@@ -232,15 +245,83 @@ class ChunkBinding:
 
     def moments(self, chunk: Chunk) -> Tuple[torch.Tensor, torch.Tensor]:
         """The flat exp_avg / exp_avg_sq of an optimizer chunk, allocated beside its shard: in device
-        memory, or in pinned host memory for a host-resident shard."""
+        memory, or in pinned host memory for a host-resident shard.  With an 8-bit state these are the
+        codes (uint8); ``scales`` has the exponents of their blocks and ``read_moments`` the values."""
         if chunk not in self.flat_m:
             if chunk.shard.is_cuda or not torch.cuda.is_available():
                 kw = dict(device=chunk.shard_device)
             else:
                 kw = dict(pin_memory=True)
-            self.flat_m[chunk] = torch.zeros(chunk.shard_size, dtype=torch.float32, **kw)
-            self.flat_v[chunk] = torch.zeros(chunk.shard_size, dtype=torch.float32, **kw)
+            dtype = torch.uint8 if self.state_bits == 8 else torch.float32
+            if self.state_bits == 8:
+                blocks = -(-chunk.shard_size // _ops_abi.STATE_BLOCK)
+                self.flat_scales[chunk] = torch.zeros(blocks, 2, dtype=torch.uint8, **kw)
+            self.flat_m[chunk] = torch.zeros(chunk.shard_size, dtype=dtype, **kw)
+            self.flat_v[chunk] = torch.zeros(chunk.shard_size, dtype=dtype, **kw)
         return self.flat_m[chunk], self.flat_v[chunk]
+
+    def scales(self, chunk: Chunk) -> torch.Tensor:
+        """The block exponents of an 8-bit state."""
+        self.moments(chunk)
+        return self.flat_scales[chunk]
+
+    def read_moments(self, chunk: Chunk, dtype: torch.dtype = torch.float32, begin: int = 0,
+                     end: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The values of exp_avg / exp_avg_sq of the elements [begin, end) of an optimizer chunk, as new
+        tensors of ``dtype``: fp32, or bf16, which also holds every value of an 8-bit state."""
+        m, v = self.moments(chunk)
+        end = m.numel() if end is None else end
+        if not 0 <= begin <= end <= m.numel():
+            raise ValueError(f'elements [{begin}, {end}) of a chunk of {m.numel()}')
+        if self.state_bits == 8:
+            return _read_state8(m, v, self.flat_scales[chunk], begin, end, dtype, self.launch_device())
+        return _as_read(m[begin:end], v[begin:end], dtype)
+
+
+_READ_DTYPES = {torch.float32: _abi.ELX_F32, torch.bfloat16: _abi.ELX_BF16}
+
+
+def _as_read(m: torch.Tensor, v: torch.Tensor, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``read_moments`` of a 32-bit state."""
+    if dtype not in _READ_DTYPES:
+        raise TypeError(f'moments are read as float32 or bfloat16, not {dtype}')
+    return m.to(dtype, copy=True), v.to(dtype, copy=True)
+
+
+def _require_reachable(*tensors: torch.Tensor) -> None:
+    if not torch.cuda.is_available() or not all(t.is_cuda or t.is_pinned() for t in tensors):
+        raise RuntimeError('HybridAdam runs on the GPU: an 8-bit state lives in device memory or in pinned host memory')
+
+
+_STATE8_PIECE = 1 << 32    # elements per launch (a call takes up to 2^33)
+
+
+def _read_state8(m: torch.Tensor, v: torch.Tensor, scales: torch.Tensor, begin: int, end: int, dtype: torch.dtype,
+                 device: torch.device) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Values of the elements [begin, end) of an 8-bit state, in device memory."""
+    if dtype not in _READ_DTYPES:
+        raise TypeError(f'moments are read as float32 or bfloat16, not {dtype}')
+    _require_reachable(m, v, scales)
+    with torch.cuda.device(device):
+        out = [torch.empty(end - begin, dtype=dtype, device=device) for _ in range(2)]
+        stream = torch.cuda.current_stream(device).cuda_stream
+        esize = out[0].element_size()
+        for b in range(begin, end, _STATE8_PIECE):
+            n = min(_STATE8_PIECE, end - b)
+            _ops_abi.state8_read(m.data_ptr(), v.data_ptr(), scales.data_ptr(), b, n,
+                                 out[0].data_ptr() + (b - begin) * esize, out[1].data_ptr() + (b - begin) * esize,
+                                 _READ_DTYPES[dtype], stream)
+    return out[0], out[1]
+
+
+def _write_state8(values: torch.Tensor, moment: int, codes: torch.Tensor, scales: torch.Tensor, device: torch.device) -> None:
+    """All of one moment (0 exp_avg, 1 exp_avg_sq) of an 8-bit state, rounded to nearest."""
+    _require_reachable(codes, scales)
+    with torch.cuda.device(device):
+        stream = torch.cuda.current_stream(device).cuda_stream
+        for b in range(0, codes.numel(), _STATE8_PIECE):    # a piece is a whole number of blocks
+            _ops_abi.state8_write(values.data_ptr() + 4 * b, min(_STATE8_PIECE, codes.numel() - b), moment,
+                                  codes.data_ptr() + b, scales.data_ptr() + 2 * (b // _ops_abi.STATE_BLOCK), stream)
 
 
 class _Prepared:
@@ -265,6 +346,10 @@ class HybridAdam(torch.optim.Optimizer):
         model_params, lr=1e-3, bias_correction=True, betas=(0.9, 0.999), eps=1e-8, weight_decay=0,
         adamw_mode=True (decoupled decay; False adds ``wd * p`` to the gradient),
         nvme_offload_fraction / nvme_offload_dir (accepted; offloading is not supported here).
+    Beyond them:
+        state_bits=32 (8: exp_avg and exp_avg_sq in 8 bits, ``state[p]['exp_avg']`` /  ``['exp_avg_sq']`` are codes
+        and ``['scales']`` the exponents of their blocks of 256; ``read_moments`` returns values, and so does
+        ``state_dict``, whose checkpoints load into either kind of state).
 
     ``step(closure=None, div_scale=-1)``: gradients are divided by ``div_scale`` when it is
     positive -- the combined loss scale and clipping coefficient of optimizer.py:166-183.
@@ -280,12 +365,16 @@ class HybridAdam(torch.optim.Optimizer):
                  adamw_mode: bool = True,
                  nvme_offload_fraction: float = 0.0,
                  nvme_offload_dir: Optional[str] = None,
+                 state_bits: int = 32,
                  **defaults):
+        if state_bits not in (8, 32):
+            raise ValueError(f'state_bits is 8 or 32, not {state_bits!r}')
         if nvme_offload_fraction != 0.0:
             raise NotImplementedError('NVMe offload of optimizer states is not supported')
         default_args = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, bias_correction=bias_correction)
         super().__init__(model_params, default_args)
         self.adamw_mode = adamw_mode
+        self.state_bits = int(state_bits)
         self.blocks_per_cu = 0    # cap on resident update workgroups per compute unit; 0: library default
         self._binding: Optional[ChunkBinding] = None
         self._plans: Dict = {}                      # plan key -> _DevicePlan
@@ -302,7 +391,7 @@ class HybridAdam(torch.optim.Optimizer):
 
     def bind_chunks(self, ranges: Dict[torch.nn.Parameter, Tuple[Chunk, int, int]]) -> ChunkBinding:
         """Called by ``ElixirOptimizer``: ``ranges[fake_param] = (optim_chunk, begin, end)``."""
-        self._binding = ChunkBinding(ranges)
+        self._binding = ChunkBinding(ranges, self.state_bits)
         self._bound_entries = None
         self._plans.clear()
         return self._binding
@@ -379,7 +468,7 @@ class HybridAdam(torch.optim.Optimizer):
         self._prepared = None
 
     def _hyper_table(self, hypers: Dict) -> np.ndarray:
-        records = [hyper_record_cached(key, self.adamw_mode) for key in hypers.keys()]
+        records = [hyper_record_cached(key, self.adamw_mode, self.state_bits) for key in hypers.keys()]
         return records[0] if len(records) == 1 else np.concatenate(records)
 
     def step(self, closure=None, div_scale: float = -1, *, gated: bool = False, defer_commit: bool = False,
@@ -450,7 +539,9 @@ class HybridAdam(torch.optim.Optimizer):
                 if 'adam_step' not in events:    # created once, recorded again every step
                     events['adam_step'] = (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
                 events['adam_step'][0].record()
-            if gated:
+            if self.state_bits == 8:
+                self._launch_state8(prep, div_scale, gated, armed_rows, together, stream)
+            elif gated:
                 rows = prep.dplan.gated_rows if armed_rows else prep.dplan.rows
                 _abi.adam_step_gated_mt(rows.ptr, len(plan.rows), prep.dplan.segs.ptr, len(plan.segs),
                                         prep.d_hypers, len(prep.hyper_host), plan.info, prep.grad_code,
@@ -482,6 +573,23 @@ class HybridAdam(torch.optim.Optimizer):
             if together and self._binding is None and prep.dplan.refresh is None:
                 self._remember_steady(prep)
         return loss
+
+    def _launch_state8(self, prep: '_Prepared', div_scale: float, gated: bool, armed_rows: bool, together: bool,
+                       stream: int) -> None:
+        """The update launch over an 8-bit state."""
+        dplan, plan = prep.dplan, prep.dplan.plan
+        rows = dplan.gated_rows if gated and armed_rows else dplan.rows
+        segs, n_segs = (dplan.segs.ptr, len(plan.segs)) if dplan.segs is not None else (None, 0)
+        head = (rows.ptr, dplan.state.ptr, len(plan.rows), segs, n_segs)
+        tail = (prep.grad_code, prep.lowp_code, self.blocks_per_cu, stream)
+        if gated:
+            _ops_abi.adam8_step_gated_mt(*head, prep.d_hypers, len(prep.hyper_host), plan.info, *tail)
+        elif together and len(prep.hyper_host) <= _abi.MAX_ARG_HYPERS:
+            _ops_abi.adam8_step_args_mt(*head, prep.hyper_host, plan.info, float(div_scale), *tail)
+        else:
+            if together:
+                _abi.put_hypers(prep.hyper_host, prep.d_hypers, stream)
+            _ops_abi.adam8_step_mt(*head, prep.d_hypers, len(prep.hyper_host), plan.info, float(div_scale), *tail)
 
     # ---- a standalone step that repeats the one before it
 
@@ -523,27 +631,30 @@ class HybridAdam(torch.optim.Optimizer):
         step = steady.step + 1
         if steady.pack is None:
             key = self._group_key(groups[steady.group_of_hyper[0]], step)
-            ptr = hyper_record_address(key, self.adamw_mode)
+            ptr = hyper_record_address(key, self.adamw_mode, self.state_bits)
             keys = (key, )
         else:
             keys = tuple(self._group_key(groups[gi], step) for gi in steady.group_of_hyper)
             # (two groups whose hyper-parameters have become equal would share a record in a freshly built plan;
             # this plan keeps one record each, which is the same arithmetic)
             for h, key in enumerate(keys):
-                steady.pack[h] = hyper_record_cached(key, self.adamw_mode)[0]
+                steady.pack[h] = hyper_record_cached(key, self.adamw_mode, self.state_bits)[0]
             ptr = steady.pack_ptr
         stream = _raw_current_stream(steady.device)
-        d_hypers = self._hyper_table_dev.reserve(len(keys) * _abi.HYPER_DTYPE.itemsize, steady.device)
-        code = steady.call(*steady.fixed, ptr, d_hypers, len(keys), *steady.tail, float(div_scale), steady.grad_code,
-                           _abi.ELX_NONE, steady.flags, self.blocks_per_cu, stream)
+        if self.state_bits == 8:
+            hypers = (ptr, len(keys))
+        else:
+            hypers = (ptr, self._hyper_table_dev.reserve(len(keys) * _abi.HYPER_DTYPE.itemsize, steady.device), len(keys))
+        code = steady.call(*steady.fixed, *hypers, *steady.tail, float(div_scale), steady.grad_code, _abi.ELX_NONE,
+                           steady.flags, self.blocks_per_cu, stream)
         if code != 0:
-            _abi.check('elx_adam_step_put_mt', code)
+            _abi.check(steady.call.__name__, code)
         # the launch is out: bookkeeping, and the records of the step after this one
         for state in steady.states:
             state['step'] = step
         steady.step = step
         for (lr, b1, b2, eps, wd, st, bc) in keys:
-            hyper_record_address((lr, b1, b2, eps, wd, st + 1, bc), self.adamw_mode)
+            hyper_record_address((lr, b1, b2, eps, wd, st + 1, bc), self.adamw_mode, self.state_bits)
 
     def commit_step(self) -> None:
         """The launched step happened: step counts advance (after the launches, so that the device is
@@ -557,7 +668,7 @@ class HybridAdam(torch.optim.Optimizer):
             self._binding.fused_writeback = True
         # the records of the next step, computed now, while the device is busy with this one
         for (lr, b1, b2, eps, wd, step, bc) in prep.hyper_keys:
-            hyper_record_cached((lr, b1, b2, eps, wd, step + 1, bc), self.adamw_mode)
+            hyper_record_cached((lr, b1, b2, eps, wd, step + 1, bc), self.adamw_mode, self.state_bits)
 
     def abort_step(self) -> None:
         """The launched step found the skip flag set on the device: nothing was updated and no step
@@ -582,6 +693,13 @@ class HybridAdam(torch.optim.Optimizer):
         detached from the flat storage; with bound chunks they are the 1-D slices this process owns."""
         self._ensure_state()
         packed = super().state_dict()
+        if self.state_bits == 8:    # values, as a 32-bit state would save them: exact, and loaded back to the same state
+            params = [p for group in self.param_groups for p in group['params']]
+            for pid, st in list(packed['state'].items()):
+                if 'scales' in st:
+                    values = dict(zip(('exp_avg', 'exp_avg_sq'), self.read_moments(params[pid])))
+                    rest = {key: value for key, value in st.items() if key != 'scales'}
+                    packed['state'][pid] = dict(rest, **{key: value.to('cpu') for key, value in values.items()})
         # torch hands out the optimizer's own per-parameter dicts: build new ones, never edit those
         packed['state'] = {
             pid: {key: (value.detach().to('cpu', copy=True) if torch.is_tensor(value) else value)
@@ -606,10 +724,12 @@ class HybridAdam(torch.optim.Optimizer):
             for key, value in sg.items():
                 if key != 'params':
                     g[key] = value
+        if self.state_bits == 8:
+            self._load_state8({id_to_param[int(pid)]: saved for pid, saved in state_dict['state'].items()})
         for pid, saved in state_dict['state'].items():
             p = id_to_param[int(pid)]
             state = self.state[p]
-            for key in ('exp_avg', 'exp_avg_sq'):
+            for key in ('exp_avg', 'exp_avg_sq') if self.state_bits == 32 else ():
                 if key not in saved:
                     continue
                 if key not in state:    # a standalone parameter that has not stepped yet
@@ -624,6 +744,73 @@ class HybridAdam(torch.optim.Optimizer):
         self._prepared = None
         self._standalone_cache = None
         self._steady = None
+
+    def read_moments(self, param: torch.nn.Parameter, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The values of (exp_avg, exp_avg_sq) of a parameter of this optimizer -- for a bound fake parameter those of
+        its slice -- as new tensors of ``dtype`` (float32 or bfloat16; both hold every value of an 8-bit state)."""
+        self._ensure_state()
+        state = self.state.get(param)
+        if not state or 'exp_avg' not in state:
+            raise ValueError('the parameter has no moments yet (or is not a parameter of this optimizer)')
+        if self.state_bits == 32:
+            return _as_read(state['exp_avg'], state['exp_avg_sq'], dtype)
+        if self._binding is not None:
+            chunk, begin, end = self._binding.ranges[param]
+            return self._binding.read_moments(chunk, dtype, begin, end)
+        m, v = _read_state8(state['exp_avg'], state['exp_avg_sq'], state['scales'], 0, param.numel(), dtype, param.device)
+        return m.view(param.shape), v.view(param.shape)
+
+    def _init_state8(self, param: torch.nn.Parameter, state: Dict) -> None:
+        """Codes and exponents of a standalone parameter: zeros."""
+        blocks = -(-param.numel() // _ops_abi.STATE_BLOCK)
+        state['exp_avg'] = torch.zeros(param.shape, dtype=torch.uint8, device=param.device)
+        state['exp_avg_sq'] = torch.zeros(param.shape, dtype=torch.uint8, device=param.device)
+        state['scales'] = torch.zeros(blocks, 2, dtype=torch.uint8, device=param.device)
+
+    @staticmethod
+    def _check_state8(param: torch.nn.Parameter, state: Dict) -> None:
+        """A state somebody has put in place by hand must be one the launches can address."""
+        n = param.numel()
+        for key, numel in (('exp_avg', n), ('exp_avg_sq', n), ('scales', 2 * -(-n // _ops_abi.STATE_BLOCK))):
+            t = state.get(key)
+            if (t is None or t.dtype != torch.uint8 or t.numel() != numel or not t.is_contiguous()
+                    or t.device != param.device):
+                raise RuntimeError(f"state['{key}'] of an 8-bit state is a contiguous uint8 tensor of {numel} elements "
+                                   f'on the device of its parameter')
+
+    def _load_state8(self, saved_of: Dict[torch.nn.Parameter, Dict]) -> None:
+        """Writes saved values into an 8-bit state.  Blocks are shared by the tensors of a chunk, so a chunk is read as a
+        whole, the saved slices are put in, and the whole is rounded once: what was saved from such a state comes back
+        without a change."""
+        keys = ('exp_avg', 'exp_avg_sq')
+        slices: Dict = {}    # (buffer) -> [(moment, begin, end, saved values)]
+        for p, saved in saved_of.items():
+            if self._binding is not None:
+                chunk, begin, end = self._binding.ranges[p]
+            else:
+                chunk, begin, end = p, 0, p.numel()
+                if any(key in saved for key in keys) and 'exp_avg' not in self.state[p] and p.numel():
+                    if p.device.type != 'cuda':
+                        raise RuntimeError('HybridAdam runs on the GPU: parameters must live in device memory')
+                    self._init_state8(p, self.state[p])
+            for moment, key in enumerate(keys):
+                if key in saved:
+                    if saved[key].numel() != end - begin:
+                        raise ValueError(f'a saved {key} has {saved[key].numel()} elements, this optimizer holds {end - begin}')
+                    if end > begin:
+                        slices.setdefault(chunk, []).append((moment, begin, end, saved[key]))
+        for chunk, parts in slices.items():
+            if self._binding is not None:
+                codes, scales, device = self._binding.moments(chunk), self._binding.scales(chunk), self._binding.launch_device()
+            else:
+                state, device = self.state[chunk], chunk.device
+                self._check_state8(chunk, state)
+                codes, scales = (state['exp_avg'], state['exp_avg_sq']), state['scales']
+            values = _read_state8(codes[0], codes[1], scales, 0, codes[0].numel(), torch.float32, device)
+            for moment, begin, end, src in parts:
+                values[moment][begin:end].copy_(src.reshape(-1))
+            for moment in {part[0] for part in parts}:
+                _write_state8(values[moment], moment, codes[moment], scales, device)
 
     def _walk_bound(self):
         """(state dict, group index, chunk index, begin, end) per bound fake parameter, in group order."""
@@ -644,6 +831,9 @@ class HybridAdam(torch.optim.Optimizer):
                     # per-tensor views of the flat moments, shaped like the optimizer's slice
                     state['exp_avg'] = flat_m[begin:end]
                     state['exp_avg_sq'] = flat_v[begin:end]
+                    if b.state_bits == 8:    # of the blocks the slice has a part in; the ends are shared with its neighbours
+                        block = _ops_abi.STATE_BLOCK
+                        state['scales'] = b.scales(chunk)[begin // block:-(-end // block)]
                 entries.append((state, gi, b.chunk_index[chunk], begin, end))
         self._bound_entries = (signature, entries)
         return entries
@@ -696,7 +886,8 @@ class HybridAdam(torch.optim.Optimizer):
                 shard_ptr = 0 if b.zero_grads else pc.shard.data_ptr()
                 out.append(FlatBuffer(grad=shard_ptr, lowp_out=shard_ptr, master=c.shard.data_ptr(),
                                       m=flat_m.data_ptr(), v=flat_v.data_ptr(), n_alloc=c.shard_size, n_valid=pc.n_valid,
-                                      segs=sorted(per_chunk[i])))
+                                      segs=sorted(per_chunk[i]),
+                                      scales=b.scales(c).data_ptr() if b.state_bits == 8 else 0, salt=i))
             return out
 
         dplan = self._device_plan(key, buffers, lowp_dtype, grad_code, lowp_code, len(hypers), device,
@@ -710,7 +901,7 @@ class HybridAdam(torch.optim.Optimizer):
         """Whether every buffer a cached walk recorded is still the one in use: parameter, gradient (address and
         dtype) and, for a parameter that has stepped, its state entry with both moments where they were."""
         states = self.state
-        for p, p_ptr, g_ptr, g_dtype, state, m_ptr, v_ptr in watch:
+        for p, p_ptr, g_ptr, g_dtype, state, m_ptr, v_ptr, s_ptr in watch:
             g = p.grad
             if g is None:
                 if g_ptr is not None:
@@ -723,12 +914,16 @@ class HybridAdam(torch.optim.Optimizer):
             m, v = state.get('exp_avg'), state.get('exp_avg_sq')
             if m is None or v is None or m.data_ptr() != m_ptr or v.data_ptr() != v_ptr:
                 return False
+            if s_ptr:
+                scales = state.get('scales')
+                if scales is None or scales.data_ptr() != s_ptr:
+                    return False
         return True
 
     def _standalone_items(self):
         """(items, gradient dtype, device) of the parameters that carry a gradient: per parameter its state
-        dict, its group index and (gradient, parameter, exp_avg, exp_avg_sq addresses, element count).  The
-        walk with its checks is repeated only when a parameter, a gradient buffer, a state entry or one of its
+        dict, its group index and (gradient, parameter, exp_avg, exp_avg_sq addresses, element count, address of
+        the block exponents of an 8-bit state or 0, place among all parameters).  The walk with its checks is repeated only when a parameter, a gradient buffer, a state entry or one of its
         moments, or the group layout has changed since the last step (every buffer is watched by address, the
         gradient by dtype too)."""
         cache = self._standalone_cache
@@ -740,10 +935,12 @@ class HybridAdam(torch.optim.Optimizer):
         items, watch = [], []
         grad_dtype = None
         device = None
+        place = -1
         for gi, group in enumerate(self.param_groups):
             for p in group['params']:
+                place += 1
                 if p.grad is None or p.numel() == 0:
-                    watch.append((p, p.data_ptr(), None, None, None, 0, 0))
+                    watch.append((p, p.data_ptr(), None, None, None, 0, 0, 0))
                     continue
                 if p.device.type != 'cuda':
                     raise RuntimeError('HybridAdam runs on the GPU: parameters must live in device memory')
@@ -759,11 +956,18 @@ class HybridAdam(torch.optim.Optimizer):
                 state = self.state[p]
                 if len(state) == 0:
                     state['step'] = 0
-                    state['exp_avg'] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                    state['exp_avg_sq'] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                    if self.state_bits == 8:
+                        self._init_state8(p, state)
+                    else:
+                        state['exp_avg'] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                        state['exp_avg_sq'] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                s_ptr = 0
+                if self.state_bits == 8:
+                    self._check_state8(p, state)
+                    s_ptr = state['scales'].data_ptr()
                 m_ptr, v_ptr = state['exp_avg'].data_ptr(), state['exp_avg_sq'].data_ptr()
-                watch.append((p, p.data_ptr(), p.grad.data_ptr(), p.grad.dtype, state, m_ptr, v_ptr))
-                items.append((state, gi, (p.grad.data_ptr(), p.data.data_ptr(), m_ptr, v_ptr, p.numel())))
+                watch.append((p, p.data_ptr(), p.grad.data_ptr(), p.grad.dtype, state, m_ptr, v_ptr, s_ptr))
+                items.append((state, gi, (p.grad.data_ptr(), p.data.data_ptr(), m_ptr, v_ptr, p.numel(), s_ptr, place)))
         result = (items, grad_dtype, device)
         self._standalone_cache = (watch, tuple(len(g['params']) for g in self.param_groups), result)
         return result
@@ -785,8 +989,9 @@ class HybridAdam(torch.optim.Optimizer):
         key = ('standalone', grad_code, tuple(it[2] for it in items), tuple(idx_of))
 
         def buffers():
-            return [FlatBuffer(grad=g, lowp_out=0, master=p, m=m, v=v, n_alloc=n, n_valid=n, segs=[(0, n, h)])
-                    for (_, _, (g, p, m, v, n)), h in zip(items, idx_of)]
+            return [FlatBuffer(grad=g, lowp_out=0, master=p, m=m, v=v, n_alloc=n, n_valid=n, segs=[(0, n, h)], scales=s,
+                               salt=place)
+                    for (_, _, (g, p, m, v, n, s, place)), h in zip(items, idx_of)]
 
         dplan = self._device_plan(key, buffers, grad_dtype, grad_code, _abi.ELX_NONE, len(hypers), device)
         return _Prepared(dplan, self._hyper_table(hypers), grad_code, _abi.ELX_NONE, device, [it[0] for it in items],

@@ -10,14 +10,16 @@ segments into
   * ``rows`` / ``segs``: the ElxChunk / ElxSeg tables of the update launch, one row per block of
     ``block_elems`` elements that contains at least one valid element;
   * ``refresh_rows``: ElxChunk rows (lowp_out, master, n_alloc only) for the padding runs, cut into
-    blocks of the same size, or None.
+    blocks of the same size, or None;
+  * ``state_rows``: for buffers whose moments are held in 8 bits, the ElxState8 row that belongs to each
+    update row (rows start at block boundaries of the code: the block is the tile), else None.
 """
 from dataclasses import dataclass, field
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 
-from . import _abi
+from . import _abi, _ops_abi
 
 MAX_ROWS = 32768    # target upper bound on update rows (the grid's y extent must stay below 65536)
 
@@ -33,6 +35,8 @@ class FlatBuffer:
     n_alloc: int
     n_valid: int
     segs: List[Tuple[int, int, int]] = field(default_factory=list)    # (begin, end, hyper), sorted, disjoint
+    scales: int = 0   # device address of the block exponents when m and v are 8-bit codes (0: m and v are fp32)
+    salt: int = 0     # with 8-bit codes: place of the buffer among the optimizer's buffers
 
 
 @dataclass
@@ -43,6 +47,7 @@ class LaunchPlan:
     refresh_max_elems: int
     block_elems: int
     info: _abi.TableInfo
+    state_rows: Optional[np.ndarray] = None
 
 
 def _pow2_at_least(x: int) -> int:
@@ -91,7 +96,10 @@ def build_plan(buffers: Sequence[FlatBuffer], grad_esize: int, lowp_esize: int, 
     memory-side cache only fronts that)."""
     tile = _abi.tile_elems()
     block = choose_block_elems(buffers, tile)
-    rows, segs, refresh = [], [], []
+    state8 = any(b.scales for b in buffers)
+    assert not state8 or all(b.scales for b in buffers), 'the moments of one launch are all in 8 bits or all in 32'
+    state_esize = 1 if state8 else 4
+    rows, segs, refresh, state_rows = [], [], [], []
     tiles = 0
     padding = sum(max(0, b.n_alloc - min(b.n_alloc, -(-b.n_valid // block) * block)) for b in buffers if b.lowp_out)
     fold = 0 < padding < fold_padding_below
@@ -116,8 +124,10 @@ def build_plan(buffers: Sequence[FlatBuffer], grad_esize: int, lowp_esize: int, 
                 for sb, se, h in seg_arr[lo:hi]:
                     segs.append((max(int(sb), b) - b, min(int(se), b + n) - b, int(h), 0))
             rows.append((buf.grad + b * grad_esize if buf.grad else 0, buf.lowp_out + b * lowp_esize if buf.lowp_out else 0,
-                         buf.master + 4 * b, buf.m + 4 * b, buf.v + 4 * b, n, max(0, min(n, buf.n_valid - b)), tiles,
-                         seg_begin, len(segs)))
+                         buf.master + 4 * b, buf.m + state_esize * b, buf.v + state_esize * b, n,
+                         max(0, min(n, buf.n_valid - b)), tiles, seg_begin, len(segs)))
+            if state8:
+                state_rows.append((buf.scales + 2 * (b // tile), b // tile, buf.salt))
             tiles += (n + tile - 1) // tile
         if buf.lowp_out:
             # the run of pure padding, in blocks of the same size: an even grid for the refresh launch
@@ -129,7 +139,7 @@ def build_plan(buffers: Sequence[FlatBuffer], grad_esize: int, lowp_esize: int, 
     info = _abi.check_tables(rows_np, segs_np, n_hypers, grad_dtype, lowp_dtype) if len(rows_np) else None
     if info is not None:
         lowp_bytes = sum(b.n_alloc for b in buffers if b.lowp_out) * lowp_esize
-        state_bytes = sum(b.n_alloc * (12 + (grad_esize if b.grad else 0)
+        state_bytes = sum(b.n_alloc * (4 + 2 * state_esize + (grad_esize if b.grad else 0)
                                        + (lowp_esize if b.lowp_out and b.lowp_out != b.grad else 0)) for b in buffers)
         policy = 0
         if device_resident and 0 < lowp_bytes <= KEEP_LOWP_CACHED_BELOW:
@@ -141,4 +151,10 @@ def build_plan(buffers: Sequence[FlatBuffer], grad_esize: int, lowp_esize: int, 
     if refresh:
         refresh_np = np.array(refresh, dtype=_abi.CHUNK_DTYPE)
         refresh_max = int(refresh_np['n_alloc'].max())
-    return LaunchPlan(rows_np, segs_np, refresh_np, refresh_max, block, info)
+    state_np = None
+    if state8:
+        assert tile == _ops_abi.STATE_BLOCK
+        state_np = np.array(state_rows, dtype=_ops_abi.STATE8_DTYPE)
+        if len(rows_np):
+            _ops_abi.check_state8(rows_np, state_np)
+    return LaunchPlan(rows_np, segs_np, refresh_np, refresh_max, block, info, state_np)
