@@ -245,7 +245,8 @@ def _prepare_chunks(case, gen):
     state = dict(case=case, step=FIRST_STEP, master=master, grads=grads, moments=moments)
     if own:
         import elixir_amd as ea
-        named = [('t%d' % i, shape) for i, shape in enumerate(_chunk_shapes(case))]
+        # a tensor that is longer than a chunk is cut to it, as the rows above are
+        named = [('t%d' % i, shape if math.prod(shape) <= size else (size, )) for i, shape in enumerate(_chunk_shapes(case))]
         module = ea.ElixirModule(dict(named), ea.greedy_search([(n, math.prod(s)) for n, s in named], size, dtype), dtype=dtype)
         inner = ea.HybridAdam(list(module.parameters()), lr=LR, betas=BETAS, eps=EPS, weight_decay=DECAY, state_bits=8)
         opt = ea.ElixirOptimizer(module, inner, initial_scale=case['loss_scale'], max_norm=case['max_norm'])
