@@ -11,9 +11,9 @@
 // (elx_kernels.hip): one tile per workgroup, tiles in address order, the number of resident workgroups held by an LDS
 // reservation that no thread touches.
 //
-// Arithmetic: fp32 as in the 32-bit update, IEEE division and square root, the fused multiply-adds written as fmaf
-// (-ffp-contract=off): a step from moments that the codes hold exactly gives the bits of the 32-bit step in master and
-// low-precision copy.  Only the new moments are rounded to 8 bits, after the master has used them.
+// Arithmetic: fp32; unscale and moments have the bits of the 32-bit update (fused multiply-adds written as fmaf,
+// -ffp-contract=off), the change of the master weight is that update's to within 2^-20.  Only the new moments are rounded to
+// 8 bits, after the master has used them.
 #include "elx_ops_device.h"
 
 #include "../elx_host.h"
@@ -31,7 +31,7 @@ constexpr uint32_t kTile = 256;
 constexpr int kVec = 4;
 static_assert(kTile == elx_host::kTile, "a tile of the update tables is a block of the 8-bit code");
 
-constexpr uint32_t kBlocksPerCu = 20;    // resident workgroups per compute unit when the caller names no number
+constexpr uint32_t kBlocksPerCu = 22;    // resident workgroups per compute unit when the caller names no number
 
 // cache policy, as in the 32-bit update: everything streams; the low-precision copy stays in the memory-side cache; all does
 enum { kStream = 0, kKeepLowp = 1, kKeepState = 2 };
@@ -67,42 +67,52 @@ __device__ __forceinline__ Hyper load_hyper(const ElxHyper *__restrict__ h) {
     return r;
 }
 
-// One element; the statements are those of the 32-bit update (torch.optim.Adam's order of operations).
-template <int MODE, bool L2, bool LERP_FROM_G>
-__device__ __forceinline__ void adam_elem(float g, float &p, float &m, float &v, const Hyper &h, const Unscale &us) {
-    if (MODE == kDivMulInv)
-        g = g * us.inv_scale;
-    else if (MODE == kDivTrue)
-        g = g / us.div_scale;
+// sqrt and reciprocal instructions (1 ulp each) stand in for the IEEE sequences: with them a launch over 1.3 billion elements
+// was bound by its vector work at any residency (3.47 ms at 32 workgroups per compute unit, 3.88 at 20), without them it is
+// bound by HBM (3.25 ms at 20, and slower again beyond 24, like a copy).  Moments and codes do not depend on them; the change of a master weight is off by at most 2^-20 of itself.  The sqrt instruction takes subnormal numbers
+// for zero: below this eps that would show, and the IEEE forms are taken.
+constexpr float kFastEps = 0x1p-36f;
+
+// One element, torch.optim.Adam's order of operations.  DIV: the gradient is divided by div_scale (else multiplied by
+// inv_scale, which is exact, and 1 when nothing is unscaled); OPTIONS: L2 decay or the lerp from the gradient's end.
+template <bool DIV, bool IEEE, bool OPTIONS>
+__device__ __forceinline__ void adam_elem(float g, float &p, float &m, float &v, const Hyper &h, const Unscale &us, float rbc2) {
+    g = DIV ? g / us.div_scale : g * us.inv_scale;
     p = p * h.decay_mul;
-    if (L2) g = fmaf(h.l2_wd, p, g);
+    if (OPTIONS && (h.flags & ELX_HYPER_L2)) g = fmaf(h.l2_wd, p, g);
     const float diff = g - m;
-    m = fmaf(h.lerp_w, diff, LERP_FROM_G ? g : m);
+    m = fmaf(h.lerp_w, diff, OPTIONS && (h.flags & ELX_HYPER_LERP_FROM_G) ? g : m);
     v = fmaf(h.omb2 * g, g, v * h.beta2);
-    const float denom = sqrtf(v) / h.bc2_sqrt + h.eps;
-    p = p + (h.neg_step * m) / denom;
+    if (IEEE) {
+        p = p + (h.neg_step * m) / (sqrtf(v) / h.bc2_sqrt + h.eps);
+    } else {
+        const float denom = fmaf(__builtin_amdgcn_sqrtf(v), rbc2, h.eps);
+        p = fmaf(h.neg_step * m, __builtin_amdgcn_rcpf(denom), p);
+    }
 }
 
-template <int MODE>
-__device__ __forceinline__ void adam_elem_flags(float g, float &p, float &m, float &v, const Hyper &h, const Unscale &us) {
-    const bool l2 = h.flags & ELX_HYPER_L2, from_g = h.flags & ELX_HYPER_LERP_FROM_G;
-    if (!l2 && !from_g)
-        adam_elem<MODE, false, false>(g, p, m, v, h, us);
-    else if (l2 && !from_g)
-        adam_elem<MODE, true, false>(g, p, m, v, h, us);
-    else if (!l2)
-        adam_elem<MODE, false, true>(g, p, m, v, h, us);
-    else
-        adam_elem<MODE, true, true>(g, p, m, v, h, us);
-}
-
-__device__ __forceinline__ void adam_elem_any(float g, float &p, float &m, float &v, const Hyper &h, const Unscale &us) {
-    if (us.mode == kDivMulInv)
-        adam_elem_flags<kDivMulInv>(g, p, m, v, h, us);
-    else if (us.mode == kDivTrue)
-        adam_elem_flags<kDivTrue>(g, p, m, v, h, us);
-    else
-        adam_elem_flags<kDivNone>(g, p, m, v, h, us);
+// calls f with the variant of adam_elem that the launch-uniform choices select
+template <typename F>
+__device__ __forceinline__ void with_variant(const Hyper &h, const Unscale &us, F &&f) {
+    const float rbc2 = __builtin_amdgcn_rcpf(h.bc2_sqrt);
+    const uint32_t kind = (us.mode == kDivTrue ? 1u : 0u) | (h.eps >= kFastEps ? 0u : 2u) |
+                          (h.flags & (ELX_HYPER_L2 | ELX_HYPER_LERP_FROM_G) ? 4u : 0u);
+#define ELX_KIND(DIV, IEEE, OPTIONS)                                                                                          \
+    case (DIV ? 1u : 0u) | (IEEE ? 2u : 0u) | (OPTIONS ? 4u : 0u):                                                            \
+        f([&](float g, float &p, float &m, float &v) { adam_elem<DIV, IEEE, OPTIONS>(g, p, m, v, h, us, rbc2); });            \
+        break;
+    switch (kind) {
+        ELX_KIND(false, false, false)
+        ELX_KIND(true, false, false)
+        ELX_KIND(false, true, false)
+        ELX_KIND(true, true, false)
+        ELX_KIND(false, false, true)
+        ELX_KIND(true, false, true)
+        ELX_KIND(false, true, true)
+        default:
+            f([&](float g, float &p, float &m, float &v) { adam_elem<true, true, true>(g, p, m, v, h, us, rbc2); });
+    }
+#undef ELX_KIND
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -126,21 +136,26 @@ __device__ __forceinline__ uint32_t dither_of(uint32_t word, int k) {
     return __builtin_rotateright32(word, 8 * k) >> 12;
 }
 
+// Lanes without a partner get 0, the identity of max: the exchange then is an operand modifier of the max itself.
 template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
-    const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, ROWS, 0xF, false);
-    return x > y ? x : y;
+__device__ __forceinline__ void dpp_max(uint32_t &x, uint32_t &y) {
+    const uint32_t a = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false);
+    const uint32_t b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)y, CTRL, ROWS, 0xF, false);
+    x = x > a ? x : a;
+    y = y > b ? y : b;
 }
-// largest of the 64 lanes, in a scalar register: inside rows of 16 (two exchanges inside quads, then of the halves of a
-// row), then each row's last lane into the row behind it, then the lower half's into the upper
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-    x = dpp_max<0xB1, 0xF>(x);     // lanes 1 0 3 2 of each quad
-    x = dpp_max<0x4E, 0xF>(x);     // lanes 2 3 0 1
-    x = dpp_max<0x141, 0xF>(x);    // mirrored within 8 lanes
-    x = dpp_max<0x140, 0xF>(x);    // mirrored within 16 lanes
-    x = dpp_max<0x142, 0xA>(x);    // lane 15 of rows 0 and 2 into rows 1 and 3
-    x = dpp_max<0x143, 0xC>(x);    // lane 31 into rows 2 and 3
-    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+// Largest of the 64 lanes, in scalar registers, for two values at a time (each exchange has to wait two instructions for
+// its operand: the other value's fill them).  Inside rows of 16 lanes: two exchanges inside quads, then of the halves of a
+// row; then each row's last lane into the row behind it, then the lower half's into the upper.
+__device__ __forceinline__ void wave_max(uint32_t &x, uint32_t &y) {
+    dpp_max<0xB1, 0xF>(x, y);     // lanes 1 0 3 2 of each quad
+    dpp_max<0x4E, 0xF>(x, y);     // lanes 2 3 0 1
+    dpp_max<0x141, 0xF>(x, y);    // mirrored within 8 lanes
+    dpp_max<0x140, 0xF>(x, y);    // mirrored within 16 lanes
+    dpp_max<0x142, 0xA>(x, y);    // lane 15 of rows 0 and 2 into rows 1 and 3
+    dpp_max<0x143, 0xC>(x, y);    // lane 31 into rows 2 and 3
+    x = (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+    y = (uint32_t)__builtin_amdgcn_readlane((int)y, 63);
 }
 
 __device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
@@ -171,55 +186,48 @@ __device__ __forceinline__ void decode_sq(uint32_t word, int e, float (&v)[kVec]
     }
 }
 
-// exp_avg of the wavefront's block -> four codes per lane and the exponent.  Called by all 64 lanes.
-__device__ __forceinline__ uint32_t encode_avg(const float (&m)[kVec], int &e) {
-    uint32_t b[kVec];
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) b[k] = magnitude(m[k]);
-    uint32_t top = wave_max(max(max(b[0], b[1]), max(b[2], b[3])));
-    const bool whole = top < kInf;
-    if (!whole) {    // the exponent is that of the finite elements
-        uint32_t t = 0;
-#pragma unroll
-        for (int k = 0; k < kVec; ++k) t = max(t, b[k] < kInf ? b[k] : 0u);
-        top = wave_max(t);
-    }
-    e = exponent_of(top);
-    float x[kVec];
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) x[k] = __builtin_ldexpf(m[k], 135 - e);
-    int word = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-    word = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], word, true);
-    if (!whole) {
-#pragma unroll
-        for (int k = 0; k < kVec; ++k)
-            if (b[k] >= kInf) word = (word & ~(0xFF << (8 * k))) | (0x7F << (8 * k));
-    }
-    return (uint32_t)word;
-}
-
-__device__ __forceinline__ uint32_t encode_sq(const float (&v)[kVec], const uint32_t (&r)[kVec], int &e) {
-    uint32_t b[kVec];
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) b[k] = magnitude(v[k]);
-    uint32_t top = wave_max(max(max(b[0], b[1]), max(b[2], b[3])));
-    const bool whole = top < kInf;
-    if (!whole) {
-        uint32_t t = 0;
-#pragma unroll
-        for (int k = 0; k < kVec; ++k) t = max(t, b[k] < kInf ? b[k] : 0u);
-        top = wave_max(t);
-    }
-    e = exponent_of(top);
-    uint32_t word = 0;
+// The moments of the wavefront's block -> four codes per lane and the two exponents.  Called by all 64 lanes.
+__device__ __forceinline__ void encode(const float (&m)[kVec], const float (&v)[kVec], const uint32_t (&r)[kVec],
+                                       uint32_t &m_word, uint32_t &v_word, int &me, int &ve) {
+    uint32_t bm[kVec], bv[kVec];
 #pragma unroll
     for (int k = 0; k < kVec; ++k) {
-        const uint32_t t = __builtin_bit_cast(uint32_t, __builtin_ldexpf(v[k], 31 - e));
-        uint32_t code = max((t + r[k]) >> 20, min(b[k], 1u));
-        if (!whole && b[k] >= kInf) code = 0xFFu;
-        word |= code << (8 * k);
+        bm[k] = magnitude(m[k]);
+        bv[k] = magnitude(v[k]);
     }
-    return word;
+    uint32_t mt = max(max(bm[0], bm[1]), max(bm[2], bm[3])), vt = max(max(bv[0], bv[1]), max(bv[2], bv[3]));
+    wave_max(mt, vt);
+    const bool whole = max(mt, vt) < kInf;
+    if (!whole) {    // the exponents are those of the finite elements
+        mt = vt = 0;
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) {
+            mt = max(mt, bm[k] < kInf ? bm[k] : 0u);
+            vt = max(vt, bv[k] < kInf ? bv[k] : 0u);
+        }
+        wave_max(mt, vt);
+    }
+    me = exponent_of(mt);
+    ve = exponent_of(vt);
+    float x[kVec];
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) x[k] = __builtin_ldexpf(m[k], 135 - me);
+    int word = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    m_word = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], word, true);
+    uint32_t code[kVec];
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+        const uint32_t t = __builtin_bit_cast(uint32_t, __builtin_ldexpf(v[k], 31 - ve));
+        code[k] = max((t + r[k]) >> 20, min(bv[k], 1u));
+    }
+    if (!whole) {
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) {
+            if (bm[k] >= kInf) m_word = (m_word & ~(0xFFu << (8 * k))) | (0x7Fu << (8 * k));
+            if (bv[k] >= kInf) code[k] = 0xFFu;
+        }
+    }
+    v_word = code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -303,7 +311,7 @@ __device__ __forceinline__ void tile_any(const Row &row, uint32_t tile, uint32_t
                 }
                 if (!GATED || !(h.gate >> 8)) {
                     const float g = c.grad ? Elem<GD>::to_f32(reinterpret_cast<const gscalar *>(c.grad)[e]) : 0.0f;
-                    adam_elem_any(g, p, m[k], v[k], h, us);
+                    with_variant(h, us, [&](auto update) { update(g, p, m[k], v[k]); });
                     c.master[e] = p;
                     r[k] = dither_of(mix(block_key(row.s.first_block + tile, row.s.salt, h.flags >> 8) + lane * kGolden), k);
                     changed = true;
@@ -316,7 +324,8 @@ __device__ __forceinline__ void tile_any(const Row &row, uint32_t tile, uint32_t
     }
     if (refresh_only || !__builtin_amdgcn_ballot_w64(changed)) return;
     int me, ve;
-    const uint32_t mw = encode_avg(m, me), vw = encode_sq(v, r, ve);
+    uint32_t mw, vw;
+    encode(m, v, r, mw, vw, me, ve);
 #pragma unroll
     for (int k = 0; k < kVec; ++k) {
         const uint32_t i = lane * kVec + k;
@@ -398,7 +407,7 @@ __device__ __forceinline__ void step_tile(const ElxChunk *__restrict__ chunks, c
             uint32_t r[kVec];
             decode_avg(mw, (int)(scales & 0xFFu), m);
             decode_sq(vw, (int)(scales >> 8), v);
-            auto elements = [&](auto update) {
+            with_variant(h, us, [&](auto update) {
 #pragma unroll
                 for (int k = 0; k < kVec; ++k) {
                     float p = P[k];
@@ -406,31 +415,10 @@ __device__ __forceinline__ void step_tile(const ElxChunk *__restrict__ chunks, c
                     P[k] = p;
                     r[k] = dither_of(word, k);
                 }
-            };
-            // the choices are uniform; each variant is straight-line code over the four elements
-            const uint32_t kind = (h.flags & (ELX_HYPER_L2 | ELX_HYPER_LERP_FROM_G)) | (uint32_t)us.mode << 2;
-#define ELX_KIND(MODE, L2, FROM_G)                                                                          \
-    case (L2 ? ELX_HYPER_L2 : 0u) | (FROM_G ? ELX_HYPER_LERP_FROM_G : 0u) | (uint32_t)MODE << 2:            \
-        elements([&](float g, float &p, float &mm, float &vv) { adam_elem<MODE, L2, FROM_G>(g, p, mm, vv, h, us); }); \
-        break;
-            switch (kind) {
-                ELX_KIND(kDivNone, false, false)
-                ELX_KIND(kDivNone, true, false)
-                ELX_KIND(kDivNone, false, true)
-                ELX_KIND(kDivNone, true, true)
-                ELX_KIND(kDivMulInv, false, false)
-                ELX_KIND(kDivMulInv, true, false)
-                ELX_KIND(kDivMulInv, false, true)
-                ELX_KIND(kDivMulInv, true, true)
-                ELX_KIND(kDivTrue, false, false)
-                ELX_KIND(kDivTrue, true, false)
-                ELX_KIND(kDivTrue, false, true)
-                default:
-                    elements([&](float g, float &p, float &mm, float &vv) { adam_elem<kDivTrue, true, true>(g, p, mm, vv, h, us); });
-            }
-#undef ELX_KIND
+            });
             int me, ve;
-            const uint32_t mo = encode_avg(m, me), vo = encode_sq(v, r, ve);
+            uint32_t mo, vo;
+            encode(m, v, r, mo, vo, me, ve);
             TileIo<f32x4>::store<Aux<POLICY>::store>(pr, lane * sizeof(f32x4), P);
             TileIo<uint32_t>::store<Aux<POLICY>::store>(mr, lane * 4, mo);
             TileIo<uint32_t>::store<Aux<POLICY>::store>(vr, lane * 4, vo);
@@ -556,8 +544,14 @@ __global__ __launch_bounds__(kStateThreads) void state8_write_kernel(const float
         x[k] = at + k < n ? values[at + k] : 0.0f;
         r[k] = kHalf;
     }
-    int e;
-    const uint32_t w = moment ? encode_sq(x, r, e) : encode_avg(x, e);
+    const float none[kVec] = {};
+    int me, ve;
+    uint32_t mw, vw;
+    if (moment)
+        encode(none, x, r, mw, vw, me, ve);
+    else
+        encode(x, none, r, mw, vw, me, ve);
+    const uint32_t w = moment ? vw : mw;
     if (at + kVec <= n) {
         *reinterpret_cast<uint32_t *>(codes + at) = w;
     } else {
@@ -565,7 +559,7 @@ __global__ __launch_bounds__(kStateThreads) void state8_write_kernel(const float
         for (int k = 0; k < kVec; ++k)
             if (at + k < n) codes[at + k] = (uint8_t)(w >> (8 * k));
     }
-    if (lane == 0) scales[2 * block + (moment ? 1 : 0)] = (uint8_t)e;
+    if (lane == 0) scales[2 * block + (moment ? 1 : 0)] = (uint8_t)(moment ? ve : me);
 }
 
 // ---------------------------------------------------------------------------------------------

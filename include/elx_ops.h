@@ -58,7 +58,8 @@ uint32_t elx_state8_block(void);
 /*
  * elx_adam_step_mt (elx_abi.h) over an 8-bit state: d_chunks as there, with m and v pointing to codes (4-byte aligned),
  * and one ElxState8 record per row in d_state.  The arithmetic on the values the codes stand for is that of
- * elx_adam_step_mt; master weights and low-precision copy come from the new moments before they are rounded.  The
+ * elx_adam_step_mt, the change of a master weight to within 2^-20 of itself (IEEE division and square root where eps is
+ * below 2^-36); master weights and low-precision copy come from the new moments before they are rounded.  The
  * rounding of exp_avg_sq takes its step from bits 8..31 of ElxHyper.flags (the step count modulo 2^24).  Elements that no
  * segment covers keep their values (to nearest, where the exponent of their block has changed).
  *   elx_adam8_step_mt        hyper records in device memory

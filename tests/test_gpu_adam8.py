@@ -1,5 +1,5 @@
-"""The Adam step over an 8-bit state on the GPU: identical bits to the oracle (oracle/state8.py over the C oracle's fp32
-step) in master weights, codes and exponents, at the sizes and values where it can go wrong."""
+"""The Adam step over an 8-bit state on the GPU against the oracle (oracle/state8.py over the C oracle's fp32 step), at the
+sizes and values where it can go wrong: identical bits in codes and exponents, master weights within ``near``."""
 import numpy as np
 import pytest
 import torch
@@ -26,6 +26,21 @@ def same_f32(got, want, what):
     nan = np.isnan(want)
     assert np.array_equal(np.isnan(got), nan), f'{what}: NaN pattern'
     assert np.array_equal(bits(got)[~nan], bits(want)[~nan]), f'{what}: {np.flatnonzero(bits(got) != bits(want))[:8]}'
+
+
+def near(got, want, before, what):
+    """Master weights after one step from the same ones (``before``).  The kernel takes the hardware's square root (1 ulp) and
+    reciprocals (1 ulp each, of the denominator and of the bias correction), with three products or sums rounded to half an
+    ulp beside them, the oracle rounds five times: relative to the change together less than 3 * 2^-23 + 8 * 2^-24 < 2^-20.
+    On top each side rounds the weight once: 2 * 2^-24 of it.  Decay is part of ``want - before``, which only widens the
+    first term.  Returns the kernel's weights, from which both sides go on."""
+    got, want, before = (np.asarray(x, np.float32).ravel() for x in (got, want, before))
+    nan = np.isnan(want)
+    assert np.array_equal(np.isnan(got), nan), f'{what}: NaN pattern'
+    g, w, b = (x[~nan].astype(np.float64) for x in (got, want, before))
+    bad = np.abs(g - w) > 2.0**-20 * np.abs(w - b) + 2.0**-23 * np.abs(w)
+    assert not bad.any(), f'{what}: {np.flatnonzero(bad)[:8]}, {np.abs(g - w).max()}'
+    return got
 
 
 def compare_codes(codes_m, codes_v, scales, want: S8.State8, what):
@@ -114,11 +129,12 @@ def test_standalone_steps_have_the_oracles_bits(oracle, adamw, wd, betas, bias):
                 p.grad.copy_(g)
         opt.step(div_scale=div)
         for i, (p, g, st) in enumerate(zip(params, grads, states)):
+            before = pn[i].copy()
             st.step(pn[i], g.numpy().copy(), O.F32, lr=1e-3, beta1=betas[0], beta2=betas[1], eps=1e-8, weight_decay=wd, step=step,
                     adamw_mode=adamw, bias_correction=bias, div_scale=div)
             got = opt.state[p]
             assert got['step'] == step
-            same_f32(to_np(p.data), pn[i], f'step {step} tensor {i} p')
+            pn[i] = near(to_np(p.data), pn[i], before, f'step {step} tensor {i} p')
             compare_codes(got['exp_avg'], got['exp_avg_sq'], got['scales'], st, f'step {step} tensor {i}')
             for t, want in zip(opt.read_moments(p), st.values()):
                 assert t.shape == p.shape
@@ -126,17 +142,22 @@ def test_standalone_steps_have_the_oracles_bits(oracle, adamw, wd, betas, bias):
     assert torch.equal(idle.data, torch.ones(5, device=DEV)) and idle not in opt.state
 
 
-def test_a_first_step_has_the_bits_of_the_32_bit_step():
-    """From moments the codes hold (zeros) the master weights are those of the 32-bit state, bit for bit."""
+@pytest.mark.parametrize('eps', [1e-8, 1e-12, 0.0])
+def test_a_first_step_is_that_of_the_32_bit_state(eps):
+    """From moments the codes hold (zeros) the master weights are those of the 32-bit state: within ``near``, and bit for bit
+    where eps is so small that the kernel divides and takes roots exactly."""
     gen = torch.Generator().manual_seed(3)
     p0, g = torch.randn(10007, generator=gen) * 0.02, torch.randn(10007, generator=gen)
+    g[:100] *= 1e-19
     out = []
     for state_bits in (8, 32):
         p = torch.nn.Parameter(p0.to(DEV))
         p.grad = g.to(DEV)
-        ea.HybridAdam([p], lr=1e-3, weight_decay=0.1, state_bits=state_bits).step()
+        ea.HybridAdam([p], lr=1e-3, weight_decay=0.1, eps=eps, state_bits=state_bits).step()
         out.append(to_np(p.data))
-    assert np.array_equal(bits(out[0]), bits(out[1]))
+    near(out[0], out[1], p0.numpy(), 'first step')
+    if eps < 2.0**-36:
+        assert np.array_equal(bits(out[0]), bits(out[1]))
 
 
 def test_gradients_that_are_not_finite(oracle):
@@ -157,9 +178,10 @@ def test_gradients_that_are_not_finite(oracle):
         g[1280] = 1e18
         p.grad = g.to(DEV)
         opt.step()
+        before = pn.copy()
         st.step(pn, g.numpy().copy(), O.F32, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0, step=step, adamw_mode=True)
         got = opt.state[p]
-        same_f32(to_np(p.data), pn, f'step {step} p')
+        pn = near(to_np(p.data), pn, before, f'step {step} p')
         compare_codes(got['exp_avg'], got['exp_avg_sq'], got['scales'], st, f'step {step}')
     m, v = opt.read_moments(p)
     assert torch.isnan(v).sum().item() == 4 and torch.isnan(m).sum().item() == 4
@@ -236,10 +258,11 @@ def test_chunked_steps_have_the_oracles_bits(oracle, dtype, graph, chunk_size):
         opt.step()
         assert opt.last_step_info['found_inf'] is False
         for i, (pc, c) in enumerate(zip(module.param_chunks, chunks)):
+            before = pn[i].copy()
             st[i].step(pn[i], grads[i], CODE[dtype], segments_of(opt, inner, c), lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, step=step,
                        adamw_mode=True, div_scale=scale if scale != 1 else -1.0)
             m, v = inner.binding.moments(c)
-            same_f32(to_np(c.shard), pn[i], f'step {step} chunk {i} master')
+            pn[i] = near(to_np(c.shard), pn[i], before, f'step {step} chunk {i} master')
             compare_codes(m, v, inner.binding.scales(c), st[i], f'step {step} chunk {i}')
             lowp = O.writeback(pn[i], CODE[dtype]) if dtype != torch.float32 else pn[i]
             assert np.array_equal(to_np(pc.shard).view(np.uint8), lowp.view(np.uint8)), f'step {step} chunk {i} writeback'
@@ -269,9 +292,11 @@ def test_a_skipped_step_leaves_the_state(gated):
 @pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
 def test_clipped_steps_follow_the_oracle(oracle, dtype):
     """With clipping the combined scale is a float64 sum in another order (1e-15 relative; the fp32 buffer of the norm can
-    turn that into one fp32 unit, 2^-23): master weights are held to the change that unit can make in the step,
-    2 * lr * 2^-23 * |update / lr| with |update / lr| <= (1 - beta1) / sqrt(1 - beta2) < 4, plus half a unit of the weight."""
+    turn that into one fp32 unit, 2^-23): master weights are held to the change that unit can make in the step, at most
+    2 * 2^-23 * |update| with |update| <= lr * (1 - beta1) / bc1 / (sqrt(1 - beta2) / sqrt(bc2)) = lr at the first step, on
+    top of what ``near`` allows."""
     module, inner, opt, gen = build8(NAMED, 5000, dtype, loss_scale=64.0 if dtype == torch.float16 else 1.0, max_norm=0.05)
+    lr = 1e-3
     scale = opt.loss_scale
     grads = land(module, opt, gen, scale, dtype)
     pn = [to_np(pc.paired_chunk.shard) for pc in module.param_chunks]
@@ -284,7 +309,7 @@ def test_clipped_steps_follow_the_oracle(oracle, dtype):
         st.step(pn[i], grads[i], CODE[dtype], segments_of(opt, inner, pc.paired_chunk), lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, step=1,
                 adamw_mode=True, div_scale=float(np.float32(combined)))
         got = to_np(pc.paired_chunk.shard)
-        assert np.all(np.abs(got - pn[i]) <= 2 * 1e-3 * 2.0**-23 * 4 + np.abs(pn[i]) * 2.0**-24), i
+        assert np.all(np.abs(got.astype(np.float64) - pn[i]) <= (2 * 2.0**-23 + 2.0**-20) * lr + np.abs(pn[i]) * 2.0**-23), i
 
 
 def test_checkpoints_resume_with_the_same_bits_and_cross_the_two_widths():
@@ -368,9 +393,10 @@ def test_shards_and_state_in_pinned_host_memory(oracle):
         for i, pc in enumerate(module.param_chunks):
             c = pc.paired_chunk
             assert all(t.is_pinned() for t in (*inner.binding.moments(c), inner.binding.scales(c)))
+            before = pn[i].copy()
             st[i].step(pn[i], grads[i], O.F16, segments_of(opt, inner, c), lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, step=step,
                        adamw_mode=True, div_scale=256.0, weight_decay=0)
-            same_f32(to_np(c.shard), pn[i], f'step {step} chunk {i}')
+            pn[i] = near(to_np(c.shard), pn[i], before, f'step {step} chunk {i}')
             compare_codes(*inner.binding.moments(c), inner.binding.scales(c), st[i], f'step {step} chunk {i}')
     assert len(opt.state_dict()['state']) == len(NAMED)
 
@@ -389,7 +415,7 @@ def test_the_allocation_step_and_many_groups(oracle):
     for i, p in enumerate(params):
         pn, st = np.full(300, 0.5, np.float32), S8.State8(300, i)
         st.step(pn, g.numpy().copy(), O.F32, lr=1e-3 * (i + 1), beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0, step=1, adamw_mode=True)
-        same_f32(to_np(p.data), pn, f'group {i}')
+        near(to_np(p.data), pn, np.full(300, 0.5, np.float32), f'group {i}')
         compare_codes(opt.state[p]['exp_avg'], opt.state[p]['exp_avg_sq'], opt.state[p]['scales'], st, f'group {i}')
 
 
@@ -413,6 +439,7 @@ def test_buffers_at_odd_offsets(oracle, odd):
     _ops_abi.check_state8(rows, state)
     dev = [torch.from_numpy(t.view(np.uint8).copy()).to(DEV) for t in (rows, state, segs)]
     pn, gn = to_np(master), to_np(grad)
+    before = pn.copy()
     _ops_abi.adam8_step_args_mt(dev[0].data_ptr(), dev[1].data_ptr(), 1, dev[2].data_ptr(), 2, hyper, info, -1.0, _abi.ELX_F16,
                                 _abi.ELX_F16, 0, torch.cuda.current_stream().cuda_stream)
     st = S8.State8(n, 9)
@@ -423,7 +450,7 @@ def test_buffers_at_odd_offsets(oracle, odd):
                 adamw_mode=True)
     finally:
         S8.dither = plain
-    same_f32(to_np(master), pn, 'master')
+    pn = near(to_np(master), pn, before, 'master')
     compare_codes(m, v, scales.view(-1, 2), st, f'odd {odd}')
     assert np.array_equal(to_np(low), O.writeback(pn, O.F16))
     for t, cut in zip(hold, (grad, low, master)):
@@ -446,9 +473,10 @@ def test_random_layouts(oracle, seed):
         opt.step()
         for i, pc in enumerate(module.param_chunks):
             c = pc.paired_chunk
+            before = pn[i].copy()
             st[i].step(pn[i], grads[i], CODE[dtype], segments_of(opt, inner, c), lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, step=step,
                        adamw_mode=True, div_scale=scale if scale != 1 else -1.0)
-            same_f32(to_np(c.shard), pn[i], f'step {step} chunk {i}')
+            pn[i] = near(to_np(c.shard), pn[i], before, f'step {step} chunk {i}')
             compare_codes(*inner.binding.moments(c), inner.binding.scales(c), st[i], f'step {step} chunk {i}')
 
 
