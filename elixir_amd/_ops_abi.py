@@ -16,7 +16,9 @@ STATE8_DTYPE = np.dtype([('scales', '<u8'), ('first_block', '<u4'), ('salt', '<u
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'libelx_ops.so')
 
 EXPORTS = ('elx_ops_version', 'elx_ops_source_sha', 'elx_sizeof_state8', 'elx_state8_block', 'elx_adam8_step_mt',
-           'elx_adam8_step_args_mt', 'elx_adam8_step_gated_mt', 'elx_check_state8', 'elx_state8_read', 'elx_state8_write')
+           'elx_adam8_step_args_mt', 'elx_adam8_step_gated_mt', 'elx_check_state8', 'elx_state8_read', 'elx_state8_write',
+           'elx_layer_norm_max_cols', 'elx_layer_norm_bwd_workspace', 'elx_layer_norm_fwd', 'elx_layer_norm_bwd',
+           'elx_embedding_fwd', 'elx_embedding_bwd_workspace', 'elx_embedding_bwd')
 
 _CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'csrc')
 _INCLUDE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'include')
@@ -67,7 +69,10 @@ def load() -> ctypes.CDLL:
     u32, u64, vp, cint, flt = ctypes.c_uint32, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_int, ctypes.c_float
     L.elx_ops_source_sha.restype = ctypes.c_char_p
     L.elx_ops_source_sha.argtypes = []
-    for name in ('elx_sizeof_state8', 'elx_state8_block'):
+    for name, args in (('elx_layer_norm_bwd_workspace', [u64, u32]), ('elx_embedding_bwd_workspace', [u64, u64, u32])):
+        getattr(L, name).restype = u64
+        getattr(L, name).argtypes = args
+    for name in ('elx_sizeof_state8', 'elx_state8_block', 'elx_layer_norm_max_cols'):
         getattr(L, name).restype = u32
         getattr(L, name).argtypes = []
     for name, args in (('elx_ops_version', []),
@@ -76,7 +81,11 @@ def load() -> ctypes.CDLL:
                        ('elx_adam8_step_args_mt', [vp, vp, u32, vp, u32, vp, u32, u64, u32, flt, cint, cint, u32, u32, vp]),
                        ('elx_adam8_step_gated_mt', [vp, vp, u32, vp, u32, vp, u32, u64, u32, cint, cint, u32, u32, vp]),
                        ('elx_state8_read', [vp, vp, vp, u64, u64, vp, vp, cint, vp]),
-                       ('elx_state8_write', [vp, u64, cint, vp, vp, vp])):
+                       ('elx_state8_write', [vp, u64, cint, vp, vp, vp]),
+                       ('elx_layer_norm_fwd', [vp, vp, vp, vp, vp, vp, u64, u32, u64, flt, cint, vp]),
+                       ('elx_layer_norm_bwd', [vp, vp, vp, vp, vp, vp, vp, vp, vp, u64, u64, u32, u64, u64, cint, vp]),
+                       ('elx_embedding_fwd', [vp, cint, u64, vp, u64, u32, flt, vp, cint, vp]),
+                       ('elx_embedding_bwd', [vp, cint, u64, vp, u64, vp, u64, u32, flt, ctypes.c_int64, vp, u64, cint, vp])):
         getattr(L, name).restype = cint
         getattr(L, name).argtypes = args
     if L.elx_ops_version() != ELX_OPS_VERSION:
@@ -141,3 +150,45 @@ def state8_read(m_codes: int, v_codes: int, scales: int, begin: int, n: int, m_o
 
 def state8_write(values: int, n: int, moment: int, codes: int, scales: int, stream: int) -> None:
     _abi.check('elx_state8_write', load().elx_state8_write(values, n, moment, codes, scales, stream))
+
+
+# ---- layer norm, embedding
+
+
+def layer_norm_max_cols() -> int:
+    return int(load().elx_layer_norm_max_cols())
+
+
+def layer_norm_bwd_workspace(rows: int, cols: int) -> int:
+    return int(load().elx_layer_norm_bwd_workspace(rows, cols))
+
+
+def layer_norm_fwd(x: int, w: int, b: int, y: int, mean: int, rstd: int, rows: int, cols: int, x_stride: int, eps: float, dtype: int,
+                   stream: int) -> None:
+    _abi.check('elx_layer_norm_fwd',
+               load().elx_layer_norm_fwd(x, w or None, b or None, y, mean or None, rstd or None, rows, cols, x_stride, eps, dtype,
+                                         stream))
+
+
+def layer_norm_bwd(dy: int, x: int, w: int, mean: int, rstd: int, dx: int, dw: int, db: int, workspace: int, workspace_bytes: int,
+                   rows: int, cols: int, dy_stride: int, x_stride: int, dtype: int, stream: int) -> None:
+    _abi.check('elx_layer_norm_bwd',
+               load().elx_layer_norm_bwd(dy, x, w or None, mean, rstd, dx or None, dw or None, db or None, workspace or None,
+                                         workspace_bytes, rows, cols, dy_stride, x_stride, dtype, stream))
+
+
+def embedding_fwd(index: int, index_bytes: int, n: int, table: int, vocab: int, cols: int, scale: float, out: int, dtype: int,
+                  stream: int) -> None:
+    _abi.check('elx_embedding_fwd',
+               load().elx_embedding_fwd(index, index_bytes, n, table, vocab, cols, scale, out, dtype, stream))
+
+
+def embedding_bwd_workspace(n: int, vocab: int, cols: int) -> int:
+    return int(load().elx_embedding_bwd_workspace(n, vocab, cols))
+
+
+def embedding_bwd(index: int, index_bytes: int, n: int, dy: int, dy_stride: int, dtable: int, vocab: int, cols: int, scale: float,
+                  padding: int, workspace: int, workspace_bytes: int, dtype: int, stream: int) -> None:
+    _abi.check('elx_embedding_bwd',
+               load().elx_embedding_bwd(index, index_bytes, n, dy, dy_stride, dtable, vocab, cols, scale, padding, workspace,
+                                        workspace_bytes, dtype, stream))

@@ -1,0 +1,491 @@
+// Layer norm over the last dimension, forward and backward (include/elx_ops.h).
+//
+//   y = (x - mean) * rstd * w + b,  mean and var over a row, rstd = 1 / sqrt(var + eps)
+//   with h = (x - mean) * rstd and t = dy * w:
+//   dx = rstd * (t - mean(t) - h * mean(t * h)),   dw = sum over rows of dy * h,   db = sum over rows of dy
+//
+// A row is held in registers from its one read to its one write: W wavefronts per row, N accesses of V elements per lane.
+// The variance is taken from the centred values in a second pass over the registers, so a large mean costs no digits.  All
+// sums are in fp32 (per lane, then inside the wavefront, then over wavefronts through LDS), the one rounding to the
+// tensor's type is at the store.
+//
+// Backward: a workgroup of 16 wavefronts has 16 / W rows in flight and walks over rows with a stride; each lane sums dw and
+// db of its own columns in registers over all its rows.  The row groups of a workgroup are added up in LDS, one partial row
+// per workgroup goes to a workspace, and a second launch adds the partial rows up in a fixed order: no atomics, the same
+// result every time.
+#include "elx_ops_device.h"
+
+using namespace elx_ops;
+
+namespace {
+
+template <int D, int V>
+struct Pack;    // V elements of type D as one access
+template <>
+struct Pack<ELX_F32, 4> {
+    typedef f32x4 type;
+};
+template <>
+struct Pack<ELX_F32, 1> {
+    typedef float type;
+};
+template <>
+struct Pack<ELX_F16, 8> {
+    typedef u16x8 type;
+};
+template <>
+struct Pack<ELX_F16, 1> {
+    typedef uint16_t type;
+};
+template <>
+struct Pack<ELX_BF16, 8> {
+    typedef u16x8 type;
+};
+template <>
+struct Pack<ELX_BF16, 1> {
+    typedef uint16_t type;
+};
+
+template <int D, int V>
+__device__ __forceinline__ void unpack(const typename Pack<D, V>::type &p, float (&x)[V]) {
+    if constexpr (V == 1) {
+        x[0] = Elem<D>::to_f32(p);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) x[k] = Elem<D>::to_f32(p[k]);
+    }
+}
+template <int D, int V>
+__device__ __forceinline__ typename Pack<D, V>::type pack(const float (&x)[V]) {
+    typename Pack<D, V>::type p;
+    if constexpr (V == 1) {
+        p = Elem<D>::from_f32(x[0]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) p[k] = Elem<D>::from_f32(x[k]);
+    }
+    return p;
+}
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_add(float x) {
+    const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xF, false);
+    return x + __builtin_bit_cast(float, y);
+}
+// sum over the 64 lanes, the same in every lane
+__device__ __forceinline__ float wave_sum(float x) {
+    x = dpp_add<0xB1, 0xF>(x);
+    x = dpp_add<0x4E, 0xF>(x);
+    x = dpp_add<0x141, 0xF>(x);
+    x = dpp_add<0x140, 0xF>(x);
+    x = dpp_add<0x142, 0xA>(x);
+    x = dpp_add<0x143, 0xC>(x);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+
+// Sum over the W wavefronts of a row; `part` is W floats of LDS that belong to this row and this sum.  Every thread of the
+// workgroup calls it.
+template <int W>
+__device__ __forceinline__ float row_sum(float x, float *part, int wave) {
+    x = wave_sum(x);
+    if constexpr (W == 1) return x;
+    if (threadIdx.x % kWave == 0) part[wave] = x;
+    __syncthreads();
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) s += part[i];
+    return s;
+}
+
+// ---------------------------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------------------------
+
+// Workgroups of max(4, W) wavefronts; with W == 1 each has a row of its own.
+template <int D, int V, int N, int W>
+__global__ __launch_bounds__(kWave *(W > 4 ? W : 4)) void layer_norm_fwd_kernel(
+    const typename Elem<D>::scalar *__restrict__ x, const typename Elem<D>::scalar *__restrict__ w,
+    const typename Elem<D>::scalar *__restrict__ b, typename Elem<D>::scalar *__restrict__ y, float *__restrict__ mean_out,
+    float *__restrict__ rstd_out, uint64_t rows, uint32_t cols, uint64_t x_stride, float eps) {
+    typedef typename Pack<D, V>::type pack_t;
+    constexpr int kGroups = W > 4 ? 1 : 4 / W;    // rows of a workgroup
+    __shared__ float part[2][kGroups][W];
+    const int wave = threadIdx.x / kWave % W, group = threadIdx.x / kWave / W, lane = threadIdx.x % kWave;
+    const uint64_t row = (uint64_t)blockIdx.x * kGroups + group;
+    const bool live = row < rows;
+    float v[N][V];
+    float s = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[n][k] = 0.0f;
+        if (live && c < cols) unpack<D, V>(__builtin_nontemporal_load(reinterpret_cast<const pack_t *>(x + row * x_stride + c)), v[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int k = 0; k < V; ++k) s += v[n][k];
+    const float inv = 1.0f / (float)cols;
+    const float mean = row_sum<W>(s, part[0][group], wave) * inv;
+    float q = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            v[n][k] -= mean;
+            if (c < cols) q = fmaf(v[n][k], v[n][k], q);
+        }
+    }
+    const float rstd = 1.0f / sqrtf(row_sum<W>(q, part[1][group], wave) * inv + eps);
+    if (!live) return;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
+        if (c < cols) {
+            float o[V], t[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) o[k] = v[n][k] * rstd;
+            if (w) {
+                unpack<D, V>(*reinterpret_cast<const pack_t *>(w + c), t);
+#pragma unroll
+                for (int k = 0; k < V; ++k) o[k] *= t[k];
+            }
+            if (b) {
+                unpack<D, V>(*reinterpret_cast<const pack_t *>(b + c), t);
+#pragma unroll
+                for (int k = 0; k < V; ++k) o[k] += t[k];
+            }
+            __builtin_nontemporal_store(pack<D, V>(o), reinterpret_cast<pack_t *>(y + row * cols + c));
+        }
+    }
+    if (wave == 0 && lane == 0) {
+        if (mean_out) mean_out[row] = mean;
+        if (rstd_out) rstd_out[row] = rstd;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------------------------
+
+constexpr int kBwdWaves = 16;
+constexpr int kBwdThreads = kBwdWaves * kWave;
+
+template <int D, int V, int N, int W>
+__global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
+    const typename Elem<D>::scalar *__restrict__ dy, const typename Elem<D>::scalar *__restrict__ x,
+    const typename Elem<D>::scalar *__restrict__ w, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
+    typename Elem<D>::scalar *__restrict__ dx, float *__restrict__ partials, uint64_t rows, uint32_t cols, uint64_t dy_stride,
+    uint64_t x_stride) {
+    typedef typename Pack<D, V>::type pack_t;
+    constexpr int kGroups = kBwdWaves / W;
+    __shared__ float part[2][2][kGroups][W];
+    const int wave = threadIdx.x / kWave % W, group = threadIdx.x / kWave / W, lane = threadIdx.x % kWave;
+    float dw[N][V], db[N][V], wt[N][V];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            dw[n][k] = db[n][k] = 0.0f;
+            wt[n][k] = 1.0f;
+        }
+        if (w && c < cols) unpack<D, V>(*reinterpret_cast<const pack_t *>(w + c), wt[n]);
+    }
+    const float inv = 1.0f / (float)cols;
+    // every wavefront takes the same number of turns: the barriers inside are the workgroup's
+    const uint64_t per_turn = (uint64_t)gridDim.x * kGroups;
+    const uint64_t turns = (rows + per_turn - 1) / per_turn;
+    for (uint64_t turn = 0; turn < turns; ++turn) {
+        const uint64_t row = turn * per_turn + (uint64_t)blockIdx.x * kGroups + group;
+        const bool live = row < rows;
+        pack_t px[N], pg[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
+            px[n] = pack_t{};
+            pg[n] = pack_t{};
+            if (live && c < cols) {
+                px[n] = __builtin_nontemporal_load(reinterpret_cast<const pack_t *>(x + row * x_stride + c));
+                pg[n] = __builtin_nontemporal_load(reinterpret_cast<const pack_t *>(dy + row * dy_stride + c));
+            }
+        }
+        const float mean = live ? mean_in[row] : 0.0f, rstd = live ? rstd_in[row] : 0.0f;
+        float h[N][V], t[N][V];
+        float st = 0.0f, sth = 0.0f;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
+            float g[V];
+            unpack<D, V>(px[n], h[n]);
+            unpack<D, V>(pg[n], g);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                h[n][k] = c < cols ? (h[n][k] - mean) * rstd : 0.0f;
+                dw[n][k] = fmaf(g[k], h[n][k], dw[n][k]);
+                db[n][k] += g[k];
+                t[n][k] = g[k] * wt[n][k];
+                st += t[n][k];
+                sth = fmaf(t[n][k], h[n][k], sth);
+            }
+        }
+        // two sums share a barrier; the buffers alternate, so a wavefront that is a turn ahead writes elsewhere
+        st = wave_sum(st);
+        sth = wave_sum(sth);
+        if constexpr (W > 1) {
+            float *p = part[turn & 1][0][group], *q = part[turn & 1][1][group];
+            if (lane == 0) {
+                p[wave] = st;
+                q[wave] = sth;
+            }
+            __syncthreads();
+            st = sth = 0.0f;
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                st += p[i];
+                sth += q[i];
+            }
+        }
+        st *= inv;
+        sth *= inv;
+        if (live && dx) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
+                if (c < cols) {
+                    float o[V];
+#pragma unroll
+                    for (int k = 0; k < V; ++k) o[k] = (t[n][k] - st - h[n][k] * sth) * rstd;
+                    __builtin_nontemporal_store(pack<D, V>(o), reinterpret_cast<pack_t *>(dx + row * cols + c));
+                }
+            }
+        }
+    }
+    if (!partials) return;
+    // add the row groups up, dw then db, through one buffer of LDS
+    __shared__ float sums[kGroups > 1 ? kGroups * W * kWave * V * N : 1];
+    constexpr uint32_t kWidth = W * kWave * V * N;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        float *out = partials + ((uint64_t)blockIdx.x * 2 + which) * cols;
+        if constexpr (kGroups > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+                    sums[group * kWidth + ((uint32_t)(n * W + wave) * kWave + lane) * V + k] = which ? db[n][k] : dw[n][k];
+            __syncthreads();
+            for (uint32_t c = threadIdx.x; c < cols; c += kBwdThreads) {
+                float s = 0.0f;
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g) s += sums[g * kWidth + c];
+                out[c] = s;
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V + k;
+                    if (c < cols) out[c] = which ? db[n][k] : dw[n][k];
+                }
+        }
+    }
+}
+
+// Adds the partial rows up: 64 columns of dw or db per workgroup, its 16 wavefronts take every 16th partial row.
+template <int D>
+__global__ __launch_bounds__(kBwdThreads) void layer_norm_fold_kernel(const float *__restrict__ partials, uint32_t blocks,
+                                                                      uint32_t cols, typename Elem<D>::scalar *dw,
+                                                                      typename Elem<D>::scalar *db) {
+    __shared__ float sums[kBwdWaves][kWave];
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const uint32_t c = blockIdx.x * kWave + lane, which = blockIdx.y;
+    float s = 0.0f;
+    if (c < cols)
+        for (uint32_t r = wave; r < blocks; r += kBwdWaves) s += partials[((uint64_t)r * 2 + which) * cols + c];
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && c < cols) {
+        s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kBwdWaves; ++i) s += sums[i][lane];
+        typename Elem<D>::scalar *out = which ? db : dw;
+        if (out) out[c] = Elem<D>::from_f32(s);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------------------------
+
+constexpr uint32_t kMaxCols = 16384;
+constexpr uint64_t kMaxRows = 1ull << 36, kMaxStride = 1ull << 36;
+constexpr uint64_t kPieceRows = 1ull << 23;
+constexpr uint32_t kBwdBlocks = 256;    // one workgroup per compute unit
+
+struct Fwd {
+    const void *x, *w, *b;
+    void *y;
+    float *mean, *rstd;
+    uint64_t rows, x_stride;
+    uint32_t cols;
+    float eps;
+    hipStream_t stream;
+};
+
+template <int D, int V, int N, int W>
+int launch_fwd(const Fwd &a) {
+    typedef typename Elem<D>::scalar T;
+    constexpr int groups = W > 4 ? 1 : 4 / W;
+    hipLaunchKernelGGL((layer_norm_fwd_kernel<D, V, N, W>), dim3((uint32_t)((a.rows + groups - 1) / groups)),
+                       dim3(kWave * (W > 4 ? W : 4)), 0, a.stream, (const T *)a.x, (const T *)a.w, (const T *)a.b, (T *)a.y, a.mean,
+                       a.rstd, a.rows, a.cols, a.x_stride, a.eps);
+    return (int)hipGetLastError();
+}
+
+// accesses per lane for `per_wave` accesses of a row per wavefront, rounded up to what is compiled
+template <int D, int V>
+int dispatch_fwd(const Fwd &a) {
+    const uint32_t accesses = (a.cols + kWave * V - 1) / (kWave * V);    // wavefront-wide accesses of a row
+    constexpr uint32_t most = 64 / V;                                    // 64 elements per lane
+    // few rows: the latency of one row counts, and four wavefronts read it in a quarter of the steps
+    if (accesses > most || (a.rows < 1024 && accesses >= 4)) {
+        const uint32_t n = (accesses + 3) / 4;
+        if (n <= 1) return launch_fwd<D, V, 1, 4>(a);
+        if (n <= 2) return launch_fwd<D, V, 2, 4>(a);
+        if (n <= 4) return launch_fwd<D, V, 4, 4>(a);
+        if constexpr (V <= 4)
+            if (n <= 16) return launch_fwd<D, V, 16, 4>(a);
+        if constexpr (V == 1) return launch_fwd<D, V, 64, 4>(a);
+        if constexpr (V > 1) return launch_fwd<D, V, most, 4>(a);
+    }
+    if (accesses <= 1) return launch_fwd<D, V, 1, 1>(a);
+    if (accesses <= 2) return launch_fwd<D, V, 2, 1>(a);
+    if (accesses <= 4) return launch_fwd<D, V, 4, 1>(a);
+    if (accesses <= 8) return launch_fwd<D, V, 8, 1>(a);
+    if constexpr (V <= 4)
+        if (accesses <= 16) return launch_fwd<D, V, 16, 1>(a);
+    if constexpr (V == 1) return launch_fwd<D, V, 64, 1>(a);
+    return ELX_E_SIZE;
+}
+
+struct Bwd {
+    const void *dy, *x, *w;
+    const float *mean, *rstd;
+    void *dx, *dw, *db;
+    float *partials;
+    uint64_t rows, dy_stride, x_stride;
+    uint32_t cols;
+    hipStream_t stream;
+};
+
+// wavefronts per row of the backward pass: at most 16 elements per lane, four where they are loaded one by one
+template <int V>
+uint32_t bwd_waves(uint32_t cols) {
+    constexpr uint32_t most = V == 1 ? 4 : 16;
+    return cols <= kWave * most ? 1 : cols <= 4 * kWave * most ? 4 : 16;
+}
+
+template <int D, int V, int N, int W>
+int launch_bwd(const Bwd &a) {
+    typedef typename Elem<D>::scalar T;
+    constexpr uint32_t groups = kBwdWaves / W;
+    const uint64_t want = (a.rows + groups - 1) / groups;
+    const uint32_t blocks = (uint32_t)(want < kBwdBlocks ? want : kBwdBlocks);
+    hipLaunchKernelGGL((layer_norm_bwd_kernel<D, V, N, W>), dim3(blocks), dim3(kBwdThreads), 0, a.stream, (const T *)a.dy,
+                       (const T *)a.x, (const T *)a.w, a.mean, a.rstd, (T *)a.dx, a.partials, a.rows, a.cols, a.dy_stride, a.x_stride);
+    if (int rc = (int)hipGetLastError()) return rc;
+    if (!a.partials) return 0;
+    hipLaunchKernelGGL((layer_norm_fold_kernel<D>), dim3((a.cols + kWave - 1) / kWave, 2), dim3(kBwdThreads), 0, a.stream, a.partials,
+                       blocks, a.cols, (T *)a.dw, (T *)a.db);
+    return (int)hipGetLastError();
+}
+
+template <int D, int V>
+int dispatch_bwd(const Bwd &a) {
+    const uint32_t waves = bwd_waves<V>(a.cols);
+    const uint32_t n = (a.cols + waves * kWave * V - 1) / (waves * kWave * V);
+#define ELX_CASE(WAVES, ACCESSES)                                                  \
+    if constexpr (ACCESSES * V <= 16)                                              \
+        if (waves == WAVES && n <= ACCESSES) return launch_bwd<D, V, ACCESSES, WAVES>(a);
+    ELX_CASE(1, 1)
+    ELX_CASE(1, 2)
+    ELX_CASE(1, 4)
+    ELX_CASE(4, 1)
+    ELX_CASE(4, 2)
+    ELX_CASE(4, 4)
+    ELX_CASE(16, 1)
+    ELX_CASE(16, 2)
+    ELX_CASE(16, 4)
+    ELX_CASE(16, 8)
+    ELX_CASE(16, 16)
+#undef ELX_CASE
+    return ELX_E_SIZE;
+}
+
+bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
+
+}    // namespace
+
+extern "C" {
+
+uint32_t elx_layer_norm_max_cols(void) { return kMaxCols; }
+
+uint64_t elx_layer_norm_bwd_workspace(uint64_t rows, uint32_t cols) {
+    const uint64_t most = rows < kBwdBlocks ? rows : kBwdBlocks;
+    return most * 2 * cols * sizeof(float);
+}
+
+int elx_layer_norm_fwd(const void *x, const void *w, const void *b, void *y, float *mean, float *rstd, uint64_t rows, uint32_t cols,
+                       uint64_t x_stride, float eps, int dtype, void *stream) {
+    if (!x || !y) return ELX_E_NULL;
+    if (!is_float_code(dtype)) return ELX_E_DTYPE;
+    if (rows == 0 || rows > kMaxRows || cols == 0 || cols > kMaxCols) return ELX_E_SIZE;
+    if ((x_stride < cols && rows > 1) || x_stride > kMaxStride) return ELX_E_RANGE;
+    const uint32_t es = elem_size(dtype), v = 16 / es;
+    if ((((uintptr_t)x | (uintptr_t)y | (uintptr_t)w | (uintptr_t)b) & (es - 1)) || (((uintptr_t)mean | (uintptr_t)rstd) & 3u))
+        return ELX_E_ALIGN;
+    const bool vec = aligned16(x) && aligned16(y) && aligned16(w) && aligned16(b) && cols % v == 0 && x_stride % v == 0;
+    // a launch has at most 2^32 threads: rows in pieces
+    for (uint64_t r = 0; r < rows; r += kPieceRows) {
+        const Fwd a = {(const char *)x + r * x_stride * es, w, b, (char *)y + r * cols * es, mean ? mean + r : nullptr,
+                       rstd ? rstd + r : nullptr, rows - r < kPieceRows ? rows - r : kPieceRows, x_stride, cols, eps,
+                       (hipStream_t)stream};
+        int rc;
+        switch (dtype) {
+            case ELX_F32: rc = vec ? dispatch_fwd<ELX_F32, 4>(a) : dispatch_fwd<ELX_F32, 1>(a); break;
+            case ELX_F16: rc = vec ? dispatch_fwd<ELX_F16, 8>(a) : dispatch_fwd<ELX_F16, 1>(a); break;
+            default: rc = vec ? dispatch_fwd<ELX_BF16, 8>(a) : dispatch_fwd<ELX_BF16, 1>(a);
+        }
+        if (rc) return rc;
+    }
+    return 0;
+}
+
+int elx_layer_norm_bwd(const void *dy, const void *x, const void *w, const float *mean, const float *rstd, void *dx, void *dw, void *db,
+                       void *workspace, uint64_t workspace_bytes, uint64_t rows, uint32_t cols, uint64_t dy_stride, uint64_t x_stride,
+                       int dtype, void *stream) {
+    if (!dy || !x || !mean || !rstd || (!dx && !dw && !db)) return ELX_E_NULL;
+    if (!is_float_code(dtype)) return ELX_E_DTYPE;
+    if (rows == 0 || rows > kMaxRows || cols == 0 || cols > kMaxCols) return ELX_E_SIZE;
+    if (((x_stride < cols || dy_stride < cols) && rows > 1) || x_stride > kMaxStride || dy_stride > kMaxStride) return ELX_E_RANGE;
+    const bool sums = dw || db;
+    if (sums && (!workspace || workspace_bytes < elx_layer_norm_bwd_workspace(rows, cols))) return !workspace ? ELX_E_NULL : ELX_E_SIZE;
+    const uint32_t es = elem_size(dtype), v = 16 / es;
+    if ((((uintptr_t)dy | (uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)db) & (es - 1)) ||
+        (((uintptr_t)mean | (uintptr_t)rstd | (uintptr_t)workspace) & 3u))
+        return ELX_E_ALIGN;
+    const Bwd a = {dy, x, w, mean, rstd, dx, dw, db, sums ? (float *)workspace : nullptr, rows, dy_stride, x_stride, cols, (hipStream_t)stream};
+    const bool vec = aligned16(dy) && aligned16(x) && aligned16(w) && aligned16(dx) && cols % v == 0 && x_stride % v == 0 && dy_stride % v == 0;
+    switch (dtype) {
+        case ELX_F32: return vec ? dispatch_bwd<ELX_F32, 4>(a) : dispatch_bwd<ELX_F32, 1>(a);
+        case ELX_F16: return vec ? dispatch_bwd<ELX_F16, 8>(a) : dispatch_bwd<ELX_F16, 1>(a);
+        default: return vec ? dispatch_bwd<ELX_BF16, 8>(a) : dispatch_bwd<ELX_BF16, 1>(a);
+    }
+}
+
+}    // extern "C"

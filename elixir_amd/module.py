@@ -17,6 +17,7 @@ import torch
 import torch.nn as nn
 
 from .chunk import Chunk, ChunkGroup, gpu_device, land_tensors
+from .fused_ops import fuse_modules
 
 
 class ChunkPlan(NamedTuple):
@@ -148,6 +149,9 @@ class ElixirModule(nn.Module):
             parameter set whose values are produced in place, directly in the chunk buffers
         search_result: chunk plans (``greedy_search`` builds one)
         dtype: the training dtype: float32, float16, or bfloat16
+        fused_ops: turn the module's ``nn.LayerNorm`` and ``nn.Embedding`` modules into ``FusedLayerNorm`` and
+            ``FusedEmbedding``, which run forward and backward on this package's kernels (results differ from torch's
+            by rounding)
     """
 
     def __init__(self,
@@ -159,7 +163,8 @@ class ElixirModule(nn.Module):
                  reduce_always_fp32: bool = False,
                  output_fp32: bool = False,
                  use_fused_kernels: bool = False,
-                 reserve_memory: bool = True) -> None:
+                 reserve_memory: bool = True,
+                 fused_ops: bool = False) -> None:
         super().__init__()
         assert dtype in {torch.float, torch.float16, torch.bfloat16}
         # Both are speed settings of the reference's forward/backward pass (module.py:51-75: overlapped chunk
@@ -170,6 +175,10 @@ class ElixirModule(nn.Module):
         self.use_fused_kernels = bool(use_fused_kernels)
 
         self.synthetic = not isinstance(module, nn.Module)
+        # fused_ops is a switch of its own: runs that pass use_fused_kernels keep their bits
+        self.fused_ops = bool(fused_ops)
+        if self.fused_ops and not self.synthetic:
+            fuse_modules(module)
         self.module = module if not self.synthetic else None
         self.dtype = dtype
         self.use_amp = (dtype == torch.float16)

@@ -2,6 +2,8 @@
  * C ABI of libelx_ops.so -- operators of a training step beside the 32-bit optimizer step, for gfx950 (MI355X):
  *
  *   adam8       Adam / AdamW over the tables of elx_abi.h with exp_avg and exp_avg_sq held in 8 bits
+ *   layer norm  forward and backward, with the reduction of the gradients of weight and bias
+ *   embedding   lookup with scaling, and the dense gradient of the table
  *
  * The conventions are those of elx_abi.h: plain C, every table pointer is a device pointer, the caller owns all
  * memory, nothing is allocated, all work goes asynchronously to the hipStream_t passed as `stream`, and every function
@@ -91,6 +93,39 @@ int elx_check_state8(const ElxChunk *h_chunks, const ElxState8 *h_state, uint32_
 int elx_state8_read(const uint8_t *m_codes, const uint8_t *v_codes, const uint16_t *scales, uint64_t begin, uint64_t n,
                     void *m_out, void *v_out, int out_dtype, void *stream);
 int elx_state8_write(const float *values, uint64_t n, int moment, uint8_t *codes, uint16_t *scales, void *stream);
+
+/*
+ * Layer norm over rows of `cols` elements (1..elx_layer_norm_max_cols()), all tensors of one type (fp32, fp16, bf16):
+ *   forward   y = (x - mean) / sqrt(var + eps) * w + b;  w and b may be NULL (1 and 0), mean and rstd (fp32, `rows` each;
+ *             what backward needs) too.  y is packed, x has rows `x_stride` elements apart.
+ *   backward  dx (packed; may be NULL), dw and db (either may be NULL).  The workspace holds one partial row of dw and
+ *             db per workgroup, elx_layer_norm_bwd_workspace() bytes, and is needed only for dw or db; contents ignored.
+ * A row is read once and written once.  Sums are in fp32; the order of every sum is fixed.
+ */
+uint32_t elx_layer_norm_max_cols(void);
+uint64_t elx_layer_norm_bwd_workspace(uint64_t rows, uint32_t cols);
+int elx_layer_norm_fwd(const void *x, const void *w, const void *b, void *y, float *mean, float *rstd, uint64_t rows,
+                       uint32_t cols, uint64_t x_stride, float eps, int dtype, void *stream);
+int elx_layer_norm_bwd(const void *dy, const void *x, const void *w, const float *mean, const float *rstd, void *dx,
+                       void *dw, void *db, void *workspace, uint64_t workspace_bytes, uint64_t rows, uint32_t cols,
+                       uint64_t dy_stride, uint64_t x_stride, int dtype, void *stream);
+
+/*
+ * Embedding of n tokens (1..2^26) in a table of `vocab` (1..2^30) rows of `cols` (1..2^20) elements of one type (fp32,
+ * fp16, bf16); indices are 4- or 8-byte integers.
+ *   forward   out[i] = scale * table[index[i]], multiplied in fp32 and rounded once.  An index outside [0, vocab) reads
+ *             nothing; its row of `out` is NaN.
+ *   backward  dtable[v] = scale * (sum of dy[i] over index[i] == v), summed in fp32 in the order of the tokens and rounded
+ *             once; rows that no token names are zero.  All of dtable is written.  Tokens whose index is `padding` (< 0:
+ *             none) or outside the table add nothing.  Rows of dy are `dy_stride` elements apart.  The workspace
+ *             (elx_embedding_bwd_workspace() bytes, 16-byte aligned, contents ignored) holds the sorted tokens and partial sums.
+ */
+int elx_embedding_fwd(const void *index, int index_bytes, uint64_t n, const void *table, uint64_t vocab, uint32_t cols,
+                      float scale, void *out, int dtype, void *stream);
+uint64_t elx_embedding_bwd_workspace(uint64_t n, uint64_t vocab, uint32_t cols);
+int elx_embedding_bwd(const void *index, int index_bytes, uint64_t n, const void *dy, uint64_t dy_stride, void *dtable,
+                      uint64_t vocab, uint32_t cols, float scale, int64_t padding, void *workspace,
+                      uint64_t workspace_bytes, int dtype, void *stream);
 
 #ifdef __cplusplus
 }
