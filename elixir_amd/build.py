@@ -1,5 +1,5 @@
 """Builds ``libelx_hip.so`` (the optimizer step) and ``libelx_ops.so`` (the operators beside it) in-tree with hipcc for
-gfx950.
+gfx950, and ``_elx_torch.so`` (autograd over the latter, host code only) with g++ against the installed torch.
 
     python -m elixir_amd.build
 
@@ -11,8 +11,9 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
-from . import _ops_abi
+from . import _ops_abi, _torch_ext
 from ._abi import LIB_PATH, built_source_sha, source_sha16
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -56,7 +57,30 @@ def build(verbose: bool = True) -> str:
             print(out)
     if failed:
         raise RuntimeError('\n'.join(failed))
+    build_torch_ext(verbose)
     return OUTPUT
+
+
+def build_torch_ext(verbose: bool = True) -> str:
+    """The Python extension with the autograd functions; links ``libelx_ops.so`` beside it."""
+    import torch
+    home = os.path.dirname(torch.__file__)
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc_path())))
+    cmd = ['g++', '-std=c++17', '-O2', '-fPIC', '-shared', '-Wall', f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}',
+           '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM', f'-DELX_TORCH_STAMP="{_torch_ext.stamp()}"',
+           '-I', os.path.join(_ROOT, 'include'), '-I', sysconfig.get_paths()['include']]
+    for path in (os.path.join(home, 'include'), os.path.join(home, 'include', 'torch', 'csrc', 'api', 'include'), os.path.join(rocm, 'include')):
+        cmd += ['-isystem', path]
+    cmd += ['-o', _torch_ext.LIB_PATH, _torch_ext.SOURCE, '-L', os.path.join(home, 'lib'), '-lc10', '-lc10_hip', '-ltorch', '-ltorch_cpu',
+            '-ltorch_hip', '-ltorch_python', '-L', _HERE, '-lelx_ops', '-Wl,-rpath,$ORIGIN']
+    if verbose:
+        print(' '.join(cmd), flush=True)
+    proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f'g++ failed ({proc.returncode}):\n{proc.stdout}')
+    if verbose and proc.stdout.strip():
+        print(proc.stdout)
+    return _torch_ext.LIB_PATH
 
 
 def build_host_checked(out_path: str, verbose: bool = False) -> str:
@@ -75,7 +99,8 @@ def build_host_checked(out_path: str, verbose: bool = False) -> str:
 def is_stale() -> bool:
     """A built library is missing, or was built from other sources than the ones beside it."""
     return (not os.path.exists(OUTPUT) or built_source_sha(OUTPUT) != source_sha16() or not os.path.exists(OPS_OUTPUT)
-            or _ops_abi.built_source_sha(OPS_OUTPUT) != _ops_abi.source_sha16())
+            or _ops_abi.built_source_sha(OPS_OUTPUT) != _ops_abi.source_sha16()
+            or _torch_ext.built_stamp(_torch_ext.LIB_PATH) != _torch_ext.stamp())
 
 
 def ensure_built(verbose: bool = False) -> str:

@@ -7,8 +7,8 @@ import torch
 from torch import nn
 
 import elixir_amd as ea
-from elixir_amd import _abi, _ops_abi
-from elixir_amd.fused_ops import _rows, fuse_modules
+from elixir_amd import _abi, _ops_abi, _torch_ext
+from elixir_amd.fused_ops import fuse_modules
 
 
 def test_functions_refuse_what_they_cannot_take():
@@ -30,6 +30,17 @@ def test_functions_refuse_what_they_cannot_take():
         ea.embedding(torch.zeros(3), table)
     with pytest.raises(ValueError, match='two dimensions'):
         ea.embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(4))
+
+
+def test_the_extension_carries_its_stamp(monkeypatch):
+    from elixir_amd import build as B
+    assert _torch_ext.built_stamp(_torch_ext.LIB_PATH) == _torch_ext.stamp() and _torch_ext.stamp() in _torch_ext.load().stamp
+    assert _torch_ext.built_stamp('/nowhere') == ''
+    monkeypatch.setattr(_torch_ext, '_ext', None)
+    monkeypatch.setattr(_torch_ext, 'stamp', lambda: 'other')
+    with pytest.raises(RuntimeError, match='built from something else'):
+        _torch_ext.load()
+    assert B.is_stale()
 
 
 def test_launches_refuse_what_they_cannot_run():
@@ -78,6 +89,7 @@ def test_launches_refuse_what_they_cannot_run():
 
 
 def test_rows_are_found_in_place_or_copied():
+    _rows = _torch_ext.load().rows_of
     base = torch.arange(240.).view(4, 5, 12)
     for x, cols, stride in ((base, 12, 12), (base[..., :8], 8, 12), (base[:, 2], 12, 60), (base[1], 12, 12), (base[::2, :, 3:7], 4, None),
                             (base.transpose(0, 1), 12, None), (base[..., ::2], 6, None), (base[0, 0].expand(3, 12), 12, None),
