@@ -120,7 +120,7 @@ __global__ __launch_bounds__(kWave *(W > 4 ? W : 4)) void layer_norm_fwd_kernel(
         const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
 #pragma unroll
         for (int k = 0; k < V; ++k) v[n][k] = 0.0f;
-        if (live && c < cols) unpack<D, V>(__builtin_nontemporal_load(reinterpret_cast<const pack_t *>(x + row * x_stride + c)), v[n]);
+        if (live && c < cols) unpack<D, V>(*reinterpret_cast<const pack_t *>(x + row * x_stride + c), v[n]);
     }
 #pragma unroll
     for (int n = 0; n < N; ++n)
@@ -170,10 +170,24 @@ __global__ __launch_bounds__(kWave *(W > 4 ? W : 4)) void layer_norm_fwd_kernel(
 // backward
 // ---------------------------------------------------------------------------------------------
 
+// The compiler may not reuse what it has computed from `x` before.
+template <typename T>
+__device__ __forceinline__ void forget(T &x) {
+    if constexpr (sizeof(T) == 16) {
+        u32x4 y = __builtin_bit_cast(u32x4, x);
+        asm volatile("" : "+v"(y));
+        x = __builtin_bit_cast(T, y);
+    }
+}
+
 constexpr int kBwdWaves = 16;
 constexpr int kBwdThreads = kBwdWaves * kWave;
+constexpr uint32_t kBwdBlocks = 256;    // one workgroup per compute unit
+// x and dy that fit the memory-side cache are likely to be there, left by the launches before: ordinary loads (8192 x 4096
+// bf16: 41 us against 47 with non-temporal ones); what does not streams past it (16384 x 4096 fp32: 135 us against 144)
+constexpr uint64_t kCacheBytes = 256ull << 20;
 
-template <int D, int V, int N, int W>
+template <int D, int V, int N, int W, bool STREAM>
 __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
     const typename Elem<D>::scalar *__restrict__ dy, const typename Elem<D>::scalar *__restrict__ x,
     const typename Elem<D>::scalar *__restrict__ w, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
@@ -181,54 +195,81 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
     uint64_t x_stride) {
     typedef typename Pack<D, V>::type pack_t;
     constexpr int kGroups = kBwdWaves / W;
+    constexpr bool kAhead = V * N <= 8;    // a lane has 128 registers: no room for a second row beyond that
     __shared__ float part[2][2][kGroups][W];
     const int wave = threadIdx.x / kWave % W, group = threadIdx.x / kWave / W, lane = threadIdx.x % kWave;
-    float dw[N][V], db[N][V], wt[N][V];
+    float dw[N][V], db[N][V];
+    pack_t pw[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
+        float one[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             dw[n][k] = db[n][k] = 0.0f;
-            wt[n][k] = 1.0f;
+            one[k] = 1.0f;
         }
-        if (w && c < cols) unpack<D, V>(*reinterpret_cast<const pack_t *>(w + c), wt[n]);
+        pw[n] = w && c < cols ? *reinterpret_cast<const pack_t *>(w + c) : pack<D, V>(one);
     }
     const float inv = 1.0f / (float)cols;
     // every wavefront takes the same number of turns: the barriers inside are the workgroup's
     const uint64_t per_turn = (uint64_t)gridDim.x * kGroups;
     const uint64_t turns = (rows + per_turn - 1) / per_turn;
-    for (uint64_t turn = 0; turn < turns; ++turn) {
+    pack_t px[N], pg[N];
+    float mean, rstd;
+    auto fetch = [&](uint64_t turn, pack_t (&qx)[N], pack_t (&qg)[N], float &m, float &r) {
         const uint64_t row = turn * per_turn + (uint64_t)blockIdx.x * kGroups + group;
         const bool live = row < rows;
-        pack_t px[N], pg[N];
+        m = live ? mean_in[row] : 0.0f;
+        r = live ? rstd_in[row] : 0.0f;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
-            px[n] = pack_t{};
-            pg[n] = pack_t{};
+            qx[n] = pack_t{};
+            qg[n] = pack_t{};
             if (live && c < cols) {
-                px[n] = __builtin_nontemporal_load(reinterpret_cast<const pack_t *>(x + row * x_stride + c));
-                pg[n] = __builtin_nontemporal_load(reinterpret_cast<const pack_t *>(dy + row * dy_stride + c));
+                const pack_t *at = reinterpret_cast<const pack_t *>(x + row * x_stride + c);
+                const pack_t *from = reinterpret_cast<const pack_t *>(dy + row * dy_stride + c);
+                if constexpr (STREAM) {
+                    qx[n] = __builtin_nontemporal_load(at);
+                    qg[n] = __builtin_nontemporal_load(from);
+                } else {
+                    qx[n] = *at;
+                    qg[n] = *from;
+                }
             }
         }
-        const float mean = live ? mean_in[row] : 0.0f, rstd = live ? rstd_in[row] : 0.0f;
-        float h[N][V], t[N][V];
+    };
+    fetch(0, px, pg, mean, rstd);
+    pack_t nx[N], ng[N];
+    float next_mean = 0.0f, next_rstd = 0.0f;
+    if constexpr (kAhead) {
+        if (turns > 1) fetch(1, nx, ng, next_mean, next_rstd);
+    }
+    for (uint64_t turn = 0; turn < turns; ++turn) {
+        const uint64_t row = turn * per_turn + (uint64_t)blockIdx.x * kGroups + group;
+        // the next two rows are on their way while this one is summed, waits at the barrier and is written
+        pack_t lx[N], lg[N];
+        float later_mean = 0.0f, later_rstd = 0.0f;
+        if constexpr (kAhead) {
+            if (turn + 2 < turns) fetch(turn + 2, lx, lg, later_mean, later_rstd);
+        }
         float st = 0.0f, sth = 0.0f;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
-            float g[V];
-            unpack<D, V>(px[n], h[n]);
+            float h[V], g[V], wt[V];
+            unpack<D, V>(px[n], h);
             unpack<D, V>(pg[n], g);
+            unpack<D, V>(pw[n], wt);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                h[n][k] = c < cols ? (h[n][k] - mean) * rstd : 0.0f;
-                dw[n][k] = fmaf(g[k], h[n][k], dw[n][k]);
+                h[k] = c < cols ? (h[k] - mean) * rstd : 0.0f;
+                dw[n][k] = fmaf(g[k], h[k], dw[n][k]);
                 db[n][k] += g[k];
-                t[n][k] = g[k] * wt[n][k];
-                st += t[n][k];
-                sth = fmaf(t[n][k], h[n][k], sth);
+                const float t = g[k] * wt[k];
+                st += t;
+                sth = fmaf(t, h[k], sth);
             }
         }
         // two sums share a barrier; the buffers alternate, so a wavefront that is a turn ahead writes elsewhere
@@ -250,17 +291,38 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
         }
         st *= inv;
         sth *= inv;
-        if (live && dx) {
+        if (row < rows && dx) {    // h and t once more, from the row as it came: cheaper than the registers to keep them
 #pragma unroll
             for (int n = 0; n < N; ++n) {
+                forget(px[n]);
+                forget(pg[n]);
+                forget(pw[n]);
                 const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
                 if (c < cols) {
-                    float o[V];
+                    float h[V], g[V], wt[V], o[V];
+                    unpack<D, V>(px[n], h);
+                    unpack<D, V>(pg[n], g);
+                    unpack<D, V>(pw[n], wt);
 #pragma unroll
-                    for (int k = 0; k < V; ++k) o[k] = (t[n][k] - st - h[n][k] * sth) * rstd;
+                    for (int k = 0; k < V; ++k) o[k] = (g[k] * wt[k] - st - (h[k] - mean) * rstd * sth) * rstd;
                     __builtin_nontemporal_store(pack<D, V>(o), reinterpret_cast<pack_t *>(dx + row * cols + c));
                 }
             }
+        }
+        if constexpr (kAhead) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                px[n] = nx[n];
+                pg[n] = ng[n];
+                nx[n] = lx[n];
+                ng[n] = lg[n];
+            }
+            mean = next_mean;
+            rstd = next_rstd;
+            next_mean = later_mean;
+            next_rstd = later_rstd;
+        } else if (turn + 1 < turns) {
+            fetch(turn + 1, px, pg, mean, rstd);
         }
     }
     if (!partials) return;
@@ -304,9 +366,15 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_fold_kernel(const floa
     __shared__ float sums[kBwdWaves][kWave];
     const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
     const uint32_t c = blockIdx.x * kWave + lane, which = blockIdx.y;
+    float x[kBwdBlocks / kBwdWaves];    // all on their way at once
+#pragma unroll
+    for (uint32_t i = 0; i < kBwdBlocks / kBwdWaves; ++i) {
+        const uint32_t r = i * kBwdWaves + wave;
+        x[i] = c < cols && r < blocks ? partials[((uint64_t)r * 2 + which) * cols + c] : 0.0f;
+    }
     float s = 0.0f;
-    if (c < cols)
-        for (uint32_t r = wave; r < blocks; r += kBwdWaves) s += partials[((uint64_t)r * 2 + which) * cols + c];
+#pragma unroll
+    for (uint32_t i = 0; i < kBwdBlocks / kBwdWaves; ++i) s += x[i];
     sums[wave][lane] = s;
     __syncthreads();
     if (wave == 0 && c < cols) {
@@ -325,7 +393,6 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_fold_kernel(const floa
 constexpr uint32_t kMaxCols = 16384;
 constexpr uint64_t kMaxRows = 1ull << 36, kMaxStride = 1ull << 36;
 constexpr uint64_t kPieceRows = 1ull << 23;
-constexpr uint32_t kBwdBlocks = 256;    // one workgroup per compute unit
 
 struct Fwd {
     const void *x, *w, *b;
@@ -352,8 +419,8 @@ template <int D, int V>
 int dispatch_fwd(const Fwd &a) {
     const uint32_t accesses = (a.cols + kWave * V - 1) / (kWave * V);    // wavefront-wide accesses of a row
     constexpr uint32_t most = 64 / V;                                    // 64 elements per lane
-    // few rows: the latency of one row counts, and four wavefronts read it in a quarter of the steps
-    if (accesses > most || (a.rows < 1024 && accesses >= 4)) {
+    // four wavefronts read a row in a quarter of the steps: for long rows, and where there are few
+    if (accesses > most || accesses >= 8 || (a.rows < 4096 && accesses >= 4)) {
         const uint32_t n = (accesses + 3) / 4;
         if (n <= 1) return launch_fwd<D, V, 1, 4>(a);
         if (n <= 2) return launch_fwd<D, V, 2, 4>(a);
@@ -383,11 +450,12 @@ struct Bwd {
     hipStream_t stream;
 };
 
-// wavefronts per row of the backward pass: at most 16 elements per lane, four where they are loaded one by one
+// wavefronts per row of the backward pass: 8 elements per lane, 4 where they are loaded one by one
 template <int V>
 uint32_t bwd_waves(uint32_t cols) {
-    constexpr uint32_t most = V == 1 ? 4 : 16;
-    return cols <= kWave * most ? 1 : cols <= 4 * kWave * most ? 4 : 16;
+    uint32_t w = 1;
+    while (w < 16 && w * kWave * (V == 1 ? 4 : 8) < cols) w *= 2;
+    return w;
 }
 
 template <int D, int V, int N, int W>
@@ -395,9 +463,17 @@ int launch_bwd(const Bwd &a) {
     typedef typename Elem<D>::scalar T;
     constexpr uint32_t groups = kBwdWaves / W;
     const uint64_t want = (a.rows + groups - 1) / groups;
-    const uint32_t blocks = (uint32_t)(want < kBwdBlocks ? want : kBwdBlocks);
-    hipLaunchKernelGGL((layer_norm_bwd_kernel<D, V, N, W>), dim3(blocks), dim3(kBwdThreads), 0, a.stream, (const T *)a.dy,
-                       (const T *)a.x, (const T *)a.w, a.mean, a.rstd, (T *)a.dx, a.partials, a.rows, a.cols, a.dy_stride, a.x_stride);
+    uint32_t blocks = (uint32_t)(want < kBwdBlocks ? want : kBwdBlocks);
+    // The partial rows of a workgroup are 16 bytes a column, written and read: where rows are few, fewer workgroups with
+    // more rows each, so that the partial rows stay below half of the tensors (300 x 11008 bf16: 31 us with 256 workgroups).
+    const uint64_t most = a.rows * sizeof(T) * 3 / 32;
+    if (a.partials && blocks > 64 && blocks > most) blocks = most < 64 ? 64 : (uint32_t)most;
+    auto kernel = layer_norm_bwd_kernel<D, V, N, W, false>;
+    if constexpr (V > 1) {
+        if (2 * a.rows * a.cols * sizeof(T) > kCacheBytes) kernel = layer_norm_bwd_kernel<D, V, N, W, true>;
+    }
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kBwdThreads), 0, a.stream, (const T *)a.dy, (const T *)a.x, (const T *)a.w, a.mean,
+                       a.rstd, (T *)a.dx, a.partials, a.rows, a.cols, a.dy_stride, a.x_stride);
     if (int rc = (int)hipGetLastError()) return rc;
     if (!a.partials) return 0;
     hipLaunchKernelGGL((layer_norm_fold_kernel<D>), dim3((a.cols + kWave - 1) / kWave, 2), dim3(kBwdThreads), 0, a.stream, a.partials,
@@ -410,14 +486,20 @@ int dispatch_bwd(const Bwd &a) {
     const uint32_t waves = bwd_waves<V>(a.cols);
     const uint32_t n = (a.cols + waves * kWave * V - 1) / (waves * kWave * V);
 #define ELX_CASE(WAVES, ACCESSES)                                                  \
-    if constexpr (ACCESSES * V <= 16)                                              \
+    if constexpr (ACCESSES * V <= (WAVES == 16 ? 16 : V == 1 ? 4 : 8))             \
         if (waves == WAVES && n <= ACCESSES) return launch_bwd<D, V, ACCESSES, WAVES>(a);
     ELX_CASE(1, 1)
     ELX_CASE(1, 2)
     ELX_CASE(1, 4)
+    ELX_CASE(2, 1)
+    ELX_CASE(2, 2)
+    ELX_CASE(2, 4)
     ELX_CASE(4, 1)
     ELX_CASE(4, 2)
     ELX_CASE(4, 4)
+    ELX_CASE(8, 1)
+    ELX_CASE(8, 2)
+    ELX_CASE(8, 4)
     ELX_CASE(16, 1)
     ELX_CASE(16, 2)
     ELX_CASE(16, 4)

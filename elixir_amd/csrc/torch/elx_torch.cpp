@@ -19,7 +19,7 @@ using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-constexpr int64_t kMaxTokens = 1ll << 26, kMaxRows = 1ll << 30, kMaxCols = 1ll << 20;    // of elx_embedding_*
+constexpr int64_t kMaxTokens = 1ll << 26, kMaxRows = 1ll << 30, kMaxCols = 1ll << 20, kMaxElems = 1ll << 34;    // of elx_embedding_*
 
 void check(const char *func, int code) { TORCH_CHECK(code == 0, func, " failed with code ", code); }
 
@@ -229,8 +229,10 @@ Tensor embedding(const Tensor &input, const Tensor &weight, const std::optional<
     check_devices("embedding", weight, input);
     check_types("embedding", weight, Tensor());
     const int64_t rows = weight.size(0), cols = weight.size(1);
-    TORCH_CHECK_VALUE(input.numel() <= kMaxTokens && rows <= kMaxRows && cols <= kMaxCols && (rows > 0 || input.numel() == 0),
-                      "embedding takes up to ", kMaxTokens, " tokens and a table of 1 to ", kMaxRows, " rows of up to ", kMaxCols, " elements");
+    TORCH_CHECK_VALUE(input.numel() <= kMaxTokens && rows <= kMaxRows && cols <= kMaxCols && (rows > 0 || input.numel() == 0) &&
+                          rows * cols <= kMaxElems && input.numel() * cols <= kMaxElems,
+                      "embedding takes up to ", kMaxTokens, " tokens and a table of 1 to ", kMaxRows, " rows of up to ", kMaxCols,
+                      " elements, at most ", kMaxElems, " elements each in the table and in the embedded tokens");
     int64_t padding = -1;
     if (padding_idx) {
         TORCH_CHECK_VALUE(*padding_idx >= -rows && *padding_idx < rows, "padding_idx ", *padding_idx, " lies outside a table of ", rows, " rows");

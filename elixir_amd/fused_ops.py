@@ -16,7 +16,7 @@ import torch.nn as nn
 from . import _ops_abi, _torch_ext
 
 _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
-_MAX_TOKENS, _MAX_ROWS, _MAX_COLS = 1 << 26, 1 << 30, 1 << 20    # of an embedding
+_MAX_TOKENS, _MAX_ROWS, _MAX_COLS, _MAX_ELEMS = 1 << 26, 1 << 30, 1 << 20, 1 << 34    # of an embedding
 _ext = None
 
 
@@ -43,7 +43,7 @@ def embedding(input: torch.Tensor, weight: torch.Tensor, padding_idx: Optional[i
     """Rows of ``weight`` named by ``input``, times ``scale`` (multiplied in fp32, rounded once).
 
     input: int64 or int32 device tensor of any shape, up to 2^26 tokens.  weight: [rows, cols] on the same device in fp32,
-        fp16 or bf16.  padding_idx: a row whose tokens add nothing to the gradient (negative: counted from the end).
+        fp16 or bf16; it and the embedded tokens have up to 2^34 elements.  padding_idx: a row whose tokens add nothing to the gradient (negative: counted from the end).
     The gradient of ``weight`` is dense, summed in fp32 in the order of the tokens (the same bits every time) and rounded
     once.  The indices are not checked on the host: one outside the table gives a row of NaN and no gradient."""
     return (_ext or _load()).embedding(input, weight, padding_idx, scale)
@@ -95,7 +95,8 @@ class FusedEmbedding(nn.Embedding):
         w = self.weight
         if (_plain_eager(input, w) and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse and w.dtype in _DTYPES
                 and input.dtype in (torch.int64, torch.int32) and w.device == input.device and input.numel() <= _MAX_TOKENS
-                and 0 < w.shape[0] <= _MAX_ROWS and w.shape[1] <= _MAX_COLS):
+                and 0 < w.shape[0] <= _MAX_ROWS and w.shape[1] <= _MAX_COLS and w.numel() <= _MAX_ELEMS
+                and input.numel() * w.shape[1] <= _MAX_ELEMS):
             return embedding(input, w, self.padding_idx, self.scale)
         out = super().forward(input)
         return out if self.scale == 1.0 else out * self.scale

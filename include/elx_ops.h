@@ -119,6 +119,7 @@ int elx_layer_norm_bwd(const void *dy, const void *x, const void *w, const float
  *             once; rows that no token names are zero.  All of dtable is written.  Tokens whose index is `padding` (< 0:
  *             none) or outside the table add nothing.  Rows of dy are `dy_stride` elements apart.  The workspace
  *             (elx_embedding_bwd_workspace() bytes, 16-byte aligned, contents ignored) holds the sorted tokens and partial sums.
+ *             n * cols and vocab * cols are at most 2^34.
  */
 int elx_embedding_fwd(const void *index, int index_bytes, uint64_t n, const void *table, uint64_t vocab, uint32_t cols,
                       float scale, void *out, int dtype, void *stream);
