@@ -1,4 +1,5 @@
-// Autograd of layer_norm and embedding over the C ABI of libelx_ops.so (include/elx_ops.h), as a Python extension.
+// Autograd of layer_norm and embedding over the C ABI of libelx_ops.so (include/elx_ops.h), as a Python extension, and the
+// reading of 8-bit moments, which a program may ask of many small tensors in turn.
 //
 // A backward pass runs on torch's own thread for the device.  A Python function called from there has to wait for the
 // interpreter to change threads and then spends tens of microseconds on its bookkeeping, more than many of these kernels
@@ -244,6 +245,29 @@ Tensor embedding(const Tensor &input, const Tensor &weight, const std::optional<
     return embedding_forward(index, weight, scale);
 }
 
+// --------------------------------------------------------------------------------------------------------- 8-bit moments
+
+// Values of the elements [begin, end) of a buffer, in the memory of `device`; codes and exponents lie there or in pinned memory.
+std::pair<Tensor, Tensor> state8_read(const Tensor &m, const Tensor &v, const Tensor &scales, int64_t begin, int64_t end, bool bf16,
+                                      int64_t device) {
+    for (const Tensor *t : {&m, &v, &scales}) {
+        TORCH_CHECK(t->is_cuda() || t->is_pinned(), "HybridAdam runs on the GPU: an 8-bit state lives in device memory or in pinned host memory");
+        TORCH_CHECK(t->scalar_type() == at::kByte && t->is_contiguous(), "an 8-bit state is held in contiguous uint8 tensors");
+    }
+    TORCH_CHECK(v.numel() == m.numel() && scales.numel() == 2 * ((m.numel() + 255) / 256) && 0 <= begin && begin <= end && end <= m.numel(),
+                "elements [", begin, ", ", end, ") of an 8-bit state of ", m.numel(), " elements");
+    const c10::Device where(at::kCUDA, (c10::DeviceIndex)device);
+    const c10::DeviceGuard guard(where);
+    const auto options = at::TensorOptions().device(where).dtype(bf16 ? at::kBFloat16 : at::kFloat);
+    const Tensor mo = at::empty({end - begin}, options), vo = at::empty({end - begin}, options);
+    const int64_t piece = 1ll << 32, es = bf16 ? 2 : 4;    // a call takes up to 2^33 elements
+    for (int64_t b = begin; b < end; b += piece)
+        check("elx_state8_read", elx_state8_read(m.data_ptr<uint8_t>(), v.data_ptr<uint8_t>(), (const uint16_t *)scales.data_ptr(), b,
+                                                 std::min(piece, end - b), (char *)mo.data_ptr() + (b - begin) * es,
+                                                 (char *)vo.data_ptr() + (b - begin) * es, bf16 ? ELX_BF16 : ELX_F32, stream_of(mo)));
+    return {mo, vo};
+}
+
 }    // namespace
 
 PYBIND11_MODULE(_elx_torch, m) {
@@ -251,4 +275,5 @@ PYBIND11_MODULE(_elx_torch, m) {
     m.def("layer_norm", &layer_norm, py::call_guard<py::gil_scoped_release>());
     m.def("embedding", &embedding, py::call_guard<py::gil_scoped_release>());
     m.def("rows_of", &rows_of);
+    m.def("state8_read", &state8_read, py::call_guard<py::gil_scoped_release>());
 }

@@ -26,7 +26,7 @@ import numpy as np
 import torch
 from torch.optim import optimizer as _torch_optimizer
 
-from . import _abi, _ops_abi
+from . import _abi, _ops_abi, _torch_ext
 from .chunk import gpu_device, Chunk, DeviceTable, dtype_code
 from .launch_plan import FlatBuffer, LaunchPlan, build_plan
 
@@ -278,7 +278,7 @@ class ChunkBinding:
         return _as_read(m[begin:end], v[begin:end], dtype)
 
 
-_READ_DTYPES = {torch.float32: _abi.ELX_F32, torch.bfloat16: _abi.ELX_BF16}
+_READ_DTYPES = (torch.float32, torch.bfloat16)
 
 
 def _as_read(m: torch.Tensor, v: torch.Tensor, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -301,17 +301,8 @@ def _read_state8(m: torch.Tensor, v: torch.Tensor, scales: torch.Tensor, begin: 
     """Values of the elements [begin, end) of an 8-bit state, in device memory."""
     if dtype not in _READ_DTYPES:
         raise TypeError(f'moments are read as float32 or bfloat16, not {dtype}')
-    _require_reachable(m, v, scales)
-    with torch.cuda.device(device):
-        out = [torch.empty(end - begin, dtype=dtype, device=device) for _ in range(2)]
-        stream = torch.cuda.current_stream(device).cuda_stream
-        esize = out[0].element_size()
-        for b in range(begin, end, _STATE8_PIECE):
-            n = min(_STATE8_PIECE, end - b)
-            _ops_abi.state8_read(m.data_ptr(), v.data_ptr(), scales.data_ptr(), b, n,
-                                 out[0].data_ptr() + (b - begin) * esize, out[1].data_ptr() + (b - begin) * esize,
-                                 _READ_DTYPES[dtype], stream)
-    return out[0], out[1]
+    return _torch_ext.load().state8_read(m, v, scales, begin, end, dtype == torch.bfloat16,
+                                          torch.cuda.current_device() if device.index is None else device.index)
 
 
 def _write_state8(values: torch.Tensor, moment: int, codes: torch.Tensor, scales: torch.Tensor, device: torch.device) -> None:
@@ -758,7 +749,7 @@ class HybridAdam(torch.optim.Optimizer):
             chunk, begin, end = self._binding.ranges[param]
             return self._binding.read_moments(chunk, dtype, begin, end)
         m, v = _read_state8(state['exp_avg'], state['exp_avg_sq'], state['scales'], 0, param.numel(), dtype, param.device)
-        return m.view(param.shape), v.view(param.shape)
+        return (m, v) if param.dim() == 1 else (m.view(param.shape), v.view(param.shape))
 
     def _init_state8(self, param: torch.nn.Parameter, state: Dict) -> None:
         """Codes and exponents of a standalone parameter: zeros."""
