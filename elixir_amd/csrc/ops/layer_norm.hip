@@ -5,6 +5,7 @@
 //   dx = rstd * (t - mean(t) - h * mean(t * h)),   dw = sum over rows of dy * h,   db = sum over rows of dy
 //
 // A row is held in registers from its one read to its one write: W wavefronts per row, N accesses of V elements per lane.
+// Short rows (a norm over the heads of attention) share a wavefront: L lanes per row, 64 / L rows.
 // The variance is taken from the centred values in a second pass over the registers, so a large mean costs no digits.  All
 // sums are in fp32 (per lane, then inside the wavefront, then over wavefronts through LDS), the one rounding to the
 // tensor's type is at the store.
@@ -72,22 +73,29 @@ __device__ __forceinline__ float dpp_add(float x) {
     const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xF, false);
     return x + __builtin_bit_cast(float, y);
 }
-// sum over the 64 lanes, the same in every lane
-__device__ __forceinline__ float wave_sum(float x) {
-    x = dpp_add<0xB1, 0xF>(x);
-    x = dpp_add<0x4E, 0xF>(x);
-    x = dpp_add<0x141, 0xF>(x);
-    x = dpp_add<0x140, 0xF>(x);
-    x = dpp_add<0x142, 0xA>(x);
-    x = dpp_add<0x143, 0xC>(x);
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+// sum over L neighbouring lanes, the same in each of them
+template <int L>
+__device__ __forceinline__ float lanes_sum(float x) {
+    if constexpr (L >= 2) x = dpp_add<0xB1, 0xF>(x);     // lanes 1 0 3 2 of each quad
+    if constexpr (L >= 4) x = dpp_add<0x4E, 0xF>(x);     // lanes 2 3 0 1
+    if constexpr (L >= 8) x = dpp_add<0x141, 0xF>(x);    // mirrored within 8
+    if constexpr (L >= 16) x = dpp_add<0x140, 0xF>(x);   // mirrored within 16
+    if constexpr (L == 32)                               // lanes 16 apart
+        x += __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, x), 0x401F));
+    if constexpr (L == 64) {
+        x = dpp_add<0x142, 0xA>(x);
+        x = dpp_add<0x143, 0xC>(x);
+        x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+    }
+    return x;
 }
 
 // Sum over the W wavefronts of a row; `part` is W floats of LDS that belong to this row and this sum.  Every thread of the
 // workgroup calls it.
-template <int W>
+template <int W, int L>
 __device__ __forceinline__ float row_sum(float x, float *part, int wave) {
-    x = wave_sum(x);
+    static_assert(W == 1 || L == kWave, "rows that share a wavefront lie in it");
+    x = lanes_sum<L>(x);
     if constexpr (W == 1) return x;
     if (threadIdx.x % kWave == 0) part[wave] = x;
     __syncthreads();
@@ -101,23 +109,24 @@ __device__ __forceinline__ float row_sum(float x, float *part, int wave) {
 // forward
 // ---------------------------------------------------------------------------------------------
 
-// Workgroups of max(4, W) wavefronts; with W == 1 each has a row of its own.
-template <int D, int V, int N, int W>
+// Workgroups of max(4, W) wavefronts; with W == 1 each has 64 / L rows of its own.
+template <int D, int V, int N, int W, int L>
 __global__ __launch_bounds__(kWave *(W > 4 ? W : 4)) void layer_norm_fwd_kernel(
     const typename Elem<D>::scalar *__restrict__ x, const typename Elem<D>::scalar *__restrict__ w,
     const typename Elem<D>::scalar *__restrict__ b, typename Elem<D>::scalar *__restrict__ y, float *__restrict__ mean_out,
     float *__restrict__ rstd_out, uint64_t rows, uint32_t cols, uint64_t x_stride, float eps) {
     typedef typename Pack<D, V>::type pack_t;
-    constexpr int kGroups = W > 4 ? 1 : 4 / W;    // rows of a workgroup
+    constexpr int kGroups = (W > 4 ? 1 : 4 / W) * (kWave / L);    // rows of a workgroup
     __shared__ float part[2][kGroups][W];
-    const int wave = threadIdx.x / kWave % W, group = threadIdx.x / kWave / W, lane = threadIdx.x % kWave;
+    const int wave = threadIdx.x / kWave % W, lane = threadIdx.x % L;
+    const int group = threadIdx.x / kWave / W * (kWave / L) + threadIdx.x % kWave / L;
     const uint64_t row = (uint64_t)blockIdx.x * kGroups + group;
     const bool live = row < rows;
     float v[N][V];
     float s = 0.0f;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
+        const uint32_t c = ((uint32_t)(n * W + wave) * L + lane) * V;
 #pragma unroll
         for (int k = 0; k < V; ++k) v[n][k] = 0.0f;
         if (live && c < cols) unpack<D, V>(*reinterpret_cast<const pack_t *>(x + row * x_stride + c), v[n]);
@@ -127,22 +136,22 @@ __global__ __launch_bounds__(kWave *(W > 4 ? W : 4)) void layer_norm_fwd_kernel(
 #pragma unroll
         for (int k = 0; k < V; ++k) s += v[n][k];
     const float inv = 1.0f / (float)cols;
-    const float mean = row_sum<W>(s, part[0][group], wave) * inv;
+    const float mean = row_sum<W, L>(s, part[0][group], wave) * inv;
     float q = 0.0f;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
+        const uint32_t c = ((uint32_t)(n * W + wave) * L + lane) * V;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             v[n][k] -= mean;
             if (c < cols) q = fmaf(v[n][k], v[n][k], q);
         }
     }
-    const float rstd = 1.0f / sqrtf(row_sum<W>(q, part[1][group], wave) * inv + eps);
+    const float rstd = 1.0f / sqrtf(row_sum<W, L>(q, part[1][group], wave) * inv + eps);
     if (!live) return;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
+        const uint32_t c = ((uint32_t)(n * W + wave) * L + lane) * V;
         if (c < cols) {
             float o[V], t[V];
 #pragma unroll
@@ -187,22 +196,23 @@ constexpr uint32_t kBwdBlocks = 256;    // one workgroup per compute unit
 // bf16: 41 us against 47 with non-temporal ones); what does not streams past it (16384 x 4096 fp32: 135 us against 144)
 constexpr uint64_t kCacheBytes = 256ull << 20;
 
-template <int D, int V, int N, int W, bool STREAM>
+template <int D, int V, int N, int W, int L, bool STREAM>
 __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
     const typename Elem<D>::scalar *__restrict__ dy, const typename Elem<D>::scalar *__restrict__ x,
     const typename Elem<D>::scalar *__restrict__ w, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
     typename Elem<D>::scalar *__restrict__ dx, float *__restrict__ partials, uint64_t rows, uint32_t cols, uint64_t dy_stride,
     uint64_t x_stride) {
     typedef typename Pack<D, V>::type pack_t;
-    constexpr int kGroups = kBwdWaves / W;
+    constexpr int kGroups = kBwdWaves / W * (kWave / L);    // rows in flight
     constexpr bool kAhead = V * N <= 8;    // a lane has 128 registers: no room for a second row beyond that
-    __shared__ float part[2][2][kGroups][W];
-    const int wave = threadIdx.x / kWave % W, group = threadIdx.x / kWave / W, lane = threadIdx.x % kWave;
+    __shared__ float part[2][2][W > 1 ? kGroups : 1][W];
+    const int wave = threadIdx.x / kWave % W, lane = threadIdx.x % L;
+    const int group = threadIdx.x / kWave / W * (kWave / L) + threadIdx.x % kWave / L;
     float dw[N][V], db[N][V];
     pack_t pw[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
+        const uint32_t c = ((uint32_t)(n * W + wave) * L + lane) * V;
         float one[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -224,7 +234,7 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
         r = live ? rstd_in[row] : 0.0f;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
+            const uint32_t c = ((uint32_t)(n * W + wave) * L + lane) * V;
             qx[n] = pack_t{};
             qg[n] = pack_t{};
             if (live && c < cols) {
@@ -257,7 +267,7 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
         float st = 0.0f, sth = 0.0f;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
+            const uint32_t c = ((uint32_t)(n * W + wave) * L + lane) * V;
             float h[V], g[V], wt[V];
             unpack<D, V>(px[n], h);
             unpack<D, V>(pg[n], g);
@@ -273,8 +283,8 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
             }
         }
         // two sums share a barrier; the buffers alternate, so a wavefront that is a turn ahead writes elsewhere
-        st = wave_sum(st);
-        sth = wave_sum(sth);
+        st = lanes_sum<L>(st);
+        sth = lanes_sum<L>(sth);
         if constexpr (W > 1) {
             float *p = part[turn & 1][0][group], *q = part[turn & 1][1][group];
             if (lane == 0) {
@@ -297,7 +307,7 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
                 forget(px[n]);
                 forget(pg[n]);
                 forget(pw[n]);
-                const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V;
+                const uint32_t c = ((uint32_t)(n * W + wave) * L + lane) * V;
                 if (c < cols) {
                     float h[V], g[V], wt[V], o[V];
                     unpack<D, V>(px[n], h);
@@ -326,24 +336,37 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
         }
     }
     if (!partials) return;
-    // add the row groups up, dw then db, through one buffer of LDS
-    __shared__ float sums[kGroups > 1 ? kGroups * W * kWave * V * N : 1];
-    constexpr uint32_t kWidth = W * kWave * V * N;
+    // rows that share a wavefront first
+#pragma unroll
+    for (int d = L; d < kWave; d <<= 1)
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                dw[n][k] += __shfl_xor(dw[n][k], d, kWave);
+                db[n][k] += __shfl_xor(db[n][k], d, kWave);
+            }
+    // add the groups of wavefronts up, dw then db, through one buffer of LDS
+    constexpr int kSums = kBwdWaves / W;
+    __shared__ float sums[kSums > 1 ? kSums * W * L * V * N : 1];
+    constexpr uint32_t kWidth = W * L * V * N;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         float *out = partials + ((uint64_t)blockIdx.x * 2 + which) * cols;
-        if constexpr (kGroups > 1) {
+        if constexpr (kSums > 1) {
             __syncthreads();
+            if (threadIdx.x % kWave < L) {
 #pragma unroll
-            for (int n = 0; n < N; ++n)
+                for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int k = 0; k < V; ++k)
-                    sums[group * kWidth + ((uint32_t)(n * W + wave) * kWave + lane) * V + k] = which ? db[n][k] : dw[n][k];
+                    for (int k = 0; k < V; ++k)
+                        sums[threadIdx.x / kWave / W * kWidth + ((uint32_t)(n * W + wave) * L + lane) * V + k] = which ? db[n][k] : dw[n][k];
+            }
             __syncthreads();
             for (uint32_t c = threadIdx.x; c < cols; c += kBwdThreads) {
                 float s = 0.0f;
 #pragma unroll
-                for (int g = 0; g < kGroups; ++g) s += sums[g * kWidth + c];
+                for (int g = 0; g < kSums; ++g) s += sums[g * kWidth + c];
                 out[c] = s;
             }
         } else {
@@ -351,7 +374,7 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
             for (int n = 0; n < N; ++n)
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
-                    const uint32_t c = ((uint32_t)(n * W + wave) * kWave + lane) * V + k;
+                    const uint32_t c = ((uint32_t)(n * W + wave) * L + lane) * V + k;
                     if (c < cols) out[c] = which ? db[n][k] : dw[n][k];
                 }
         }
@@ -404,11 +427,11 @@ struct Fwd {
     hipStream_t stream;
 };
 
-template <int D, int V, int N, int W>
+template <int D, int V, int N, int W, int L = kWave>
 int launch_fwd(const Fwd &a) {
     typedef typename Elem<D>::scalar T;
-    constexpr int groups = W > 4 ? 1 : 4 / W;
-    hipLaunchKernelGGL((layer_norm_fwd_kernel<D, V, N, W>), dim3((uint32_t)((a.rows + groups - 1) / groups)),
+    constexpr int groups = (W > 4 ? 1 : 4 / W) * (kWave / L);
+    hipLaunchKernelGGL((layer_norm_fwd_kernel<D, V, N, W, L>), dim3((uint32_t)((a.rows + groups - 1) / groups)),
                        dim3(kWave * (W > 4 ? W : 4)), 0, a.stream, (const T *)a.x, (const T *)a.w, (const T *)a.b, (T *)a.y, a.mean,
                        a.rstd, a.rows, a.cols, a.x_stride, a.eps);
     return (int)hipGetLastError();
@@ -430,6 +453,10 @@ int dispatch_fwd(const Fwd &a) {
         if constexpr (V == 1) return launch_fwd<D, V, 64, 4>(a);
         if constexpr (V > 1) return launch_fwd<D, V, most, 4>(a);
     }
+    if (a.cols <= 4 * V) return launch_fwd<D, V, 1, 1, 4>(a);
+    if (a.cols <= 8 * V) return launch_fwd<D, V, 1, 1, 8>(a);
+    if (a.cols <= 16 * V) return launch_fwd<D, V, 1, 1, 16>(a);
+    if (a.cols <= 32 * V) return launch_fwd<D, V, 1, 1, 32>(a);
     if (accesses <= 1) return launch_fwd<D, V, 1, 1>(a);
     if (accesses <= 2) return launch_fwd<D, V, 2, 1>(a);
     if (accesses <= 4) return launch_fwd<D, V, 4, 1>(a);
@@ -458,19 +485,19 @@ uint32_t bwd_waves(uint32_t cols) {
     return w;
 }
 
-template <int D, int V, int N, int W>
+template <int D, int V, int N, int W, int L = kWave>
 int launch_bwd(const Bwd &a) {
     typedef typename Elem<D>::scalar T;
-    constexpr uint32_t groups = kBwdWaves / W;
+    constexpr uint32_t groups = kBwdWaves / W * (kWave / L);
     const uint64_t want = (a.rows + groups - 1) / groups;
     uint32_t blocks = (uint32_t)(want < kBwdBlocks ? want : kBwdBlocks);
     // The partial rows of a workgroup are 16 bytes a column, written and read: where rows are few, fewer workgroups with
     // more rows each, so that the partial rows stay below half of the tensors (300 x 11008 bf16: 31 us with 256 workgroups).
     const uint64_t most = a.rows * sizeof(T) * 3 / 32;
     if (a.partials && blocks > 64 && blocks > most) blocks = most < 64 ? 64 : (uint32_t)most;
-    auto kernel = layer_norm_bwd_kernel<D, V, N, W, false>;
+    auto kernel = layer_norm_bwd_kernel<D, V, N, W, L, false>;
     if constexpr (V > 1) {
-        if (2 * a.rows * a.cols * sizeof(T) > kCacheBytes) kernel = layer_norm_bwd_kernel<D, V, N, W, true>;
+        if (2 * a.rows * a.cols * sizeof(T) > kCacheBytes) kernel = layer_norm_bwd_kernel<D, V, N, W, L, true>;
     }
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kBwdThreads), 0, a.stream, (const T *)a.dy, (const T *)a.x, (const T *)a.w, a.mean,
                        a.rstd, (T *)a.dx, a.partials, a.rows, a.cols, a.dy_stride, a.x_stride);
@@ -483,6 +510,10 @@ int launch_bwd(const Bwd &a) {
 
 template <int D, int V>
 int dispatch_bwd(const Bwd &a) {
+    if (a.cols <= 4 * V) return launch_bwd<D, V, 1, 1, 4>(a);
+    if (a.cols <= 8 * V) return launch_bwd<D, V, 1, 1, 8>(a);
+    if (a.cols <= 16 * V) return launch_bwd<D, V, 1, 1, 16>(a);
+    if (a.cols <= 32 * V) return launch_bwd<D, V, 1, 1, 32>(a);
     const uint32_t waves = bwd_waves<V>(a.cols);
     const uint32_t n = (a.cols + waves * kWave * V - 1) / (waves * kWave * V);
 #define ELX_CASE(WAVES, ACCESSES)                                                  \

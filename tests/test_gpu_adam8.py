@@ -505,3 +505,46 @@ def test_moments_follow_the_gradients_over_many_steps():
     m, v = opt.read_moments(p)
     assert abs(v.mean().item() / mean / 0.999**1000 - 1) < 0.03, v.mean().item() / mean
     assert m.abs().max().item() < 1e-3
+
+
+def test_a_buffer_of_more_than_2_to_the_32_elements(oracle):
+    """One parameter whose offsets pass 32 bits.  Every 2^20 elements hold the same values, so master weights and the codes of
+    exp_avg are those of one such stretch; exp_avg_sq is rounded by its place and is one of the two codes around its value.
+    The last stretch, cut short, against the oracle."""
+    stretch, n = 1 << 20, (1 << 32) + (1 << 20) + 77
+    gen = torch.Generator().manual_seed(4)
+    p0, g0 = torch.randn(stretch, generator=gen) * 0.02, torch.randn(stretch, generator=gen) * 1e-2
+    reps = -(-n // stretch)
+    p = torch.nn.Parameter(p0.to(DEV).repeat(reps)[:n].clone())
+    p.grad = g0.to(DEV).repeat(reps)[:n].clone()
+    opt = ea.HybridAdam([p], lr=1e-3, weight_decay=0.1, state_bits=8)
+    opt.step()
+    st = S8.State8(stretch, 0)
+    pn = p0.numpy().copy()
+    st.step(pn, g0.numpy().copy(), O.F32, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.1, step=1, adamw_mode=True)
+    first = p.data[:stretch]
+    near(to_np(first), pn, p0.numpy(), 'first stretch')
+    whole = p.data[:n - n % stretch].view(-1, stretch)
+    assert torch.equal(whole, first.expand_as(whole)) and torch.equal(p.data[n - n % stretch:], first[:n % stretch])
+    codes = opt.state[p]['exp_avg']
+    assert np.array_equal(to_np(codes[:stretch]), st.m.reshape(-1))
+    tail = n - n % stretch
+    assert torch.equal(codes[(1 << 32):(1 << 32) + stretch], codes[:stretch])
+    # the last block is cut short: its exponent may be another, so the values of its neighbours are compared
+    assert torch.equal(codes[tail - 256:tail], codes[stretch - 256:stretch])
+    m, v = opt.read_moments(p)
+    assert torch.equal(m[(1 << 32) - 1000:(1 << 32) + 1000], m[:stretch].roll(1000)[:2000])
+    v32 = np.float32(1.0 - 0.999) * g0.numpy() * g0.numpy()
+    lo, hi = S8.decode_sq(*S8.encode_sq(S8.to_blocks(v32), np.zeros((stretch // 256, 256), np.int64))), \
+        S8.decode_sq(*S8.encode_sq(S8.to_blocks(v32), np.full((stretch // 256, 256), (1 << 20) - 1, np.int64)))
+    got = to_np(v[(1 << 32):(1 << 32) + stretch])
+    slack = 2.0**-20    # the product above is rounded once less than the kernel's
+    assert np.all(got >= lo.reshape(-1) * (1 - slack) - 1e-30) and np.all(got <= hi.reshape(-1) * (1 + slack) + 1e-30)
+    block = (1 << 32) // 256 + 5    # and the dither of a block beyond 2^32 elements
+    g = g0.numpy()[5 * 256:6 * 256]
+    vv = np.zeros(256, np.float32)
+    O.adam(g.copy(), O.F32, p0.numpy()[5 * 256:6 * 256].copy(), np.zeros(256, np.float32), vv, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8,
+           weight_decay=0.1, step=1, adamw_mode=True)
+    want, e = S8.encode_sq(vv[None], S8.dither(np.array([block]), 0, 1))
+    assert np.array_equal(to_np(opt.state[p]['exp_avg_sq'][block * 256:(block + 1) * 256]), want[0])
+    assert to_np(opt.state[p]['scales'])[block, 1] == e[0]

@@ -208,6 +208,53 @@ def test_streams_and_graphs():
         assert all(torch.equal(a, e) for a, e in zip(out, eager)), seed
 
 
+def test_two_graphs_do_not_share_a_workspace():
+    graphs = []
+    for seed, (tokens, vocab) in enumerate(((6000, 300), (900, 2000))):
+        index, table, dy = make(tokens, vocab, 64, torch.float32, seed=seed)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(index, table, dy)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(index, table, dy)
+        graphs.append((graph, out, (index, table, dy)))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for (graph, _, _), stream in zip(graphs, streams):    # both in flight
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, out, (index, table, dy) in graphs:
+        assert all(torch.equal(a, e) for a, e in zip(out, run(index, table.detach().clone(), dy)))
+
+
+def test_a_table_of_more_than_2_to_the_31_elements():
+    """Offsets that pass 32 bits in the table, its gradient and the embedded tokens."""
+    vocab, cols = 2**20 + 40000, 2048
+    table = torch.zeros(vocab, cols, dtype=torch.float16, device=DEV)
+    rows = torch.tensor([0, 5, 2**19, 2**20 - 1, 2**20, 2**20 + 1, vocab - 1], device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    table[rows] = torch.randn(len(rows), cols, generator=g, device=DEV).half()
+    index = rows[torch.randint(0, len(rows), (2**20 + 9000, ), generator=g, device=DEV)]
+    dy = torch.zeros(len(index), cols, dtype=torch.float16, device=DEV)
+    at = torch.tensor([0, 3, 2**20 - 1, 2**20, 2**20 + 1, len(index) - 1], device=DEV)
+    dy[at] = torch.randn(len(at), cols, generator=g, device=DEV).half()
+    table.requires_grad_()
+    y = ea.embedding(index, table)
+    assert torch.equal(y[at], table.detach()[index[at]]) and torch.equal(y[2**20 + 5], table.detach()[index[2**20 + 5]])
+    d, = torch.autograd.grad(y, table, dy)
+    want = torch.zeros(len(rows), cols, dtype=torch.float64, device=DEV)
+    for i in at.tolist():
+        want[(rows == index[i]).nonzero().item()] += dy[i].double()
+    # at most six numbers that are not zero in a sum, so at most six roundings
+    assert torch.all((d[rows].double() - want).abs() <= half_step(torch.float16, want) + 6 * 2.0**-24 * 6 * dy.abs().max().item())
+    assert d.abs().sum(dtype=torch.float64).item() == d[rows].abs().sum(dtype=torch.float64).item()
+
+
 def test_the_module_runs_the_kernel_and_falls_back(monkeypatch):
     from elixir_amd import fused_ops
     calls = []

@@ -9,7 +9,8 @@ the way of one element into a row sum (64 per lane or 16 per lane, 6 across lane
     dx              rstd u (4 |t| + (K + 4) mean|t| + |h| (K + 4) mean|t h|) + rstd (|h| mean(|t| dh) + dh mean|t h|)
                     + (K / 2 + 8) u |dx|, and half a step
     dw, db          sum |dy| dh + R u sum |dy h| and R u sum |dy|, and half a step, where R = rows / 256 + 64 additions: a
-                    lane's own rows (at least 256 workgroups share them), then 16 row groups, 16 and 16 partial rows
+                    lane's own rows (256 workgroups share them; fewer only where a workgroup then has at most 6), then 6 across
+                    lanes, 16 row groups, 16 and 16 partial rows
 An extra factor of 2 covers what is of second order in u."""
 import pytest
 import torch
@@ -92,7 +93,8 @@ def test_every_width(rows, cols, dtype):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
-@pytest.mark.parametrize('rows,cols', [(2047, 769), (4096, 64), (1023, 2048), (1025, 4096), (20000, 24), (8192, 1024), (5000, 1000)])
+@pytest.mark.parametrize('rows,cols', [(2047, 769), (4096, 64), (1023, 2048), (1025, 4096), (20000, 24), (8192, 1024), (5000, 1000),
+                                       (70001, 128), (30000, 8), (30001, 17), (700, 11008)])
 def test_many_rows(rows, cols, dtype):
     x, w, b, dy = inputs(rows, cols, dtype, seed=rows)
     got = dict(zip(('y', 'dx', 'dw', 'db'), run(x, w, b, dy)))
@@ -274,6 +276,66 @@ def test_streams_and_graphs():
         eager = run(nx, nw, nb, ng)
         torch.cuda.synchronize()
         assert all(torch.equal(a, e) for a, e in zip(out, eager)), seed
+
+
+def test_two_graphs_do_not_share_a_workspace():
+    graphs = []
+    for seed, (rows, cols) in enumerate(((700, 512), (300, 2048))):
+        args = [t.detach() for t in inputs(rows, cols, torch.float32, seed=seed)]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(*args)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(*args)
+        graphs.append((graph, out, args))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for (graph, _, _), stream in zip(graphs, streams):    # both in flight
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, out, args in graphs:
+        assert all(torch.equal(a, e) for a, e in zip(out, run(*[t.detach().clone() for t in args])))
+
+
+def test_saved_tensor_hooks_checkpointing_and_anomaly_mode():
+    """What calls back into Python from inside the extension."""
+    x, w, b, dy = inputs(40, 96, torch.float32)
+    want = run(x.clone(), w.clone(), b.clone(), dy)
+    leaves = [t.detach().clone().requires_grad_() for t in (x, w, b)]
+    with torch.autograd.graph.save_on_cpu():
+        y = ea.layer_norm(*leaves)
+    assert all(torch.equal(a, e) for a, e in zip(torch.autograd.grad(y, leaves, dy), want[1:]))
+    y = torch.utils.checkpoint.checkpoint(ea.layer_norm, *leaves, use_reentrant=False)
+    assert all(torch.equal(a, e) for a, e in zip(torch.autograd.grad(y, leaves, dy), want[1:]))
+    with torch.autograd.set_detect_anomaly(True):
+        assert all(torch.equal(a, e) for a, e in zip(torch.autograd.grad(ea.layer_norm(*leaves), leaves, dy), want[1:]))
+    with torch.inference_mode():
+        assert torch.equal(ea.layer_norm(x, w, b), want[0])
+
+
+def test_more_than_2_to_the_32_elements():
+    """Rows whose offsets pass 32 bits, in elements and in bytes; the last and some in between against float64."""
+    rows, cols = 2**31 // 1024 + 2**31 // 1024 + 3, 1024
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    pick = torch.tensor([0, 1, 2**21 - 1, 2**21, 2**21 + 1, 2**22 - 1, 2**22, rows - 1], device=DEV)
+    x.zero_()
+    x[pick] = torch.randn(len(pick), cols, generator=g, device=DEV).bfloat16()
+    w, b = (1 + 0.1 * torch.randn(cols, generator=g, device=DEV)).bfloat16(), torch.randn(cols, generator=g, device=DEV).bfloat16()
+    dy = torch.zeros_like(x)
+    dy[pick] = torch.randn(len(pick), cols, generator=g, device=DEV).bfloat16()
+    y, dx, dw, db = run(x, w, b, dy)
+    ref = reference(x[pick], w, b, dy[pick], 1e-5, torch.bfloat16)
+    check(y[pick], *ref['y'], 'y')
+    check(dx[pick], *ref['dx'], 'dx')
+    check(dw, *ref['dw'], 'dw')    # rows of zeros add nothing
+    check(db, *ref['db'], 'db')
+    assert torch.equal(y[5], b) and torch.equal(y[2**22 + 1], b) and not dx[2**22 + 1].any()
 
 
 def test_the_module_runs_the_kernel_and_falls_back(monkeypatch):
