@@ -8,8 +8,10 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/autograd.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "elx_ops.h"
@@ -32,11 +34,27 @@ void *stream_of(const Tensor &t) {
     return (void *)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
 }
 
-void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+// NULL for a tensor that is not there -- and for no other: a tensor without memory of its own (a wrapper) is refused
+void *ptr(const Tensor &t) {
+    if (!t.defined()) return nullptr;
+    void *p = t.data_ptr();
+    TORCH_CHECK(p || t.numel() == 0, "a tensor without memory");
+    return p;
+}
+
+// A transform that would see the allocations of a call but not its launches must not record it.
+void check_transforms(const char *name, std::initializer_list<const Tensor *> tensors) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() &&
+                                    !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+                                name, " cannot be traced");
+    for (const Tensor *t : tensors)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), name, " has no forward-mode derivative");
+}
 
 // `x` as rows of `cols` elements: the tensor to read them from and the distance of two rows.  A tensor whose rows do not
 // lie at one distance, or whose elements do not lie side by side, is copied.
-std::pair<Tensor, int64_t> rows_of(const Tensor &x, int64_t cols) {
+std::pair<Tensor, int64_t> rows_of(const Tensor &any, int64_t cols) {
+    const Tensor x = any.resolve_neg();
     if (x.is_contiguous()) return {x, cols};
     const int64_t dims = x.dim();
     if (dims >= 1 && x.size(-1) == cols && (x.stride(-1) == 1 || cols == 1)) {
@@ -56,6 +74,14 @@ std::pair<Tensor, int64_t> rows_of(const Tensor &x, int64_t cols) {
         if (even) return {x, step == 0 ? cols : step};
     }
     return {x.contiguous(), cols};
+}
+
+Tensor packed(const Tensor &t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
+
+// What a hook on the saved tensors hands back is laid out as what it was given.
+void check_saved(const char *name, const Tensor &t, c10::ScalarType type, const c10::Device &device, int64_t numel) {
+    TORCH_CHECK(t.scalar_type() == type && t.device() == device && t.numel() == numel, name, ": a saved tensor came back as ", t.numel(),
+                " elements of ", c10::getDtypeNames(t.scalar_type()).first, " on ", t.device());
 }
 
 void check_devices(const char *name, const Tensor &first, const Tensor &other) {
@@ -78,9 +104,9 @@ Tensor layer_norm_forward(const Tensor &x, const Tensor &weight, const Tensor &b
     const int64_t rows = x.numel() / cols;
     if (rows == 0) return y;
     const auto [src, stride] = rows_of(x, cols);
-    const Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
+    const Tensor w = packed(weight), b = packed(bias);
     float *mean = stats.defined() ? stats.data_ptr<float>() : nullptr;
-    check("elx_layer_norm_fwd", elx_layer_norm_fwd(src.data_ptr(), ptr(w), ptr(b), y.data_ptr(), mean, mean ? mean + rows : nullptr, rows,
+    check("elx_layer_norm_fwd", elx_layer_norm_fwd(ptr(src), ptr(w), ptr(b), ptr(y), mean, mean ? mean + rows : nullptr, rows,
                                                    (uint32_t)cols, stride, (float)eps, code_of(x), stream_of(x)));
     return y;
 }
@@ -99,11 +125,16 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
+        const Tensor &x = saved[0], &weight = saved[1], stats = packed(saved[2]);
+        const Tensor &grad = grads[0];
         const int64_t dims = ctx->saved_data["dims"].toInt(), affine = ctx->saved_data["affine"].toInt();
-        const c10::DeviceGuard guard(x.device());
-        const auto shape = x.sizes().slice(x.dim() - dims);
+        const c10::DeviceGuard guard(grad.device());
+        const auto shape = grad.sizes().slice(grad.dim() - dims);
+        check_saved("layer_norm", x, grad.scalar_type(), grad.device(), grad.numel());
+        if (weight.defined()) check_saved("layer_norm", weight, grad.scalar_type(), grad.device(), c10::multiply_integers(shape));
+        TORCH_CHECK(x.sizes() == grad.sizes(), "layer_norm: a saved tensor came back in another shape");
         const int64_t cols = c10::multiply_integers(shape), rows = x.numel() / cols;
+        check_saved("layer_norm", stats, at::kFloat, grad.device(), 2 * rows);
         size_t edge = 0;    // inputs that are not there have no edge
         const bool want_x = ctx->needs_input_grad(edge++);
         const bool want_w = (affine & 1) && ctx->needs_input_grad(edge++);
@@ -116,7 +147,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
             if (want_w) leaves.push_back(weight);
             if (want_b) leaves.push_back(b);
             const Tensor y = at::layer_norm(x, shape, weight, b, ctx->saved_data["eps"].toDouble());
-            auto got = torch::autograd::grad({y}, leaves, {grads[0]}, std::nullopt, true);
+            auto got = torch::autograd::grad({y}, leaves, {grad}, std::nullopt, true);
             size_t i = 0;
             if (want_x) dx = got[i++];
             if (want_w) dw = got[i++];
@@ -131,14 +162,14 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
             if (want_b) db.zero_();
         } else if (want_x || want_w || want_b) {
             const auto [src, x_stride] = rows_of(x, cols);
-            const auto [dy, dy_stride] = rows_of(grads[0], cols);
-            const Tensor w = weight.defined() ? weight.contiguous() : weight;
+            const auto [dy, dy_stride] = rows_of(grad, cols);
+            const Tensor w = packed(weight);
             Tensor workspace;
             const uint64_t bytes = want_w || want_b ? elx_layer_norm_bwd_workspace(rows, (uint32_t)cols) : 0;
             if (bytes) workspace = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
             const float *mean = stats.data_ptr<float>();
             check("elx_layer_norm_bwd",
-                  elx_layer_norm_bwd(dy.data_ptr(), src.data_ptr(), ptr(w), mean, mean + rows, ptr(dx), ptr(dw), ptr(db), ptr(workspace),
+                  elx_layer_norm_bwd(ptr(dy), ptr(src), ptr(w), mean, mean + rows, ptr(dx), ptr(dw), ptr(db), ptr(workspace),
                                      bytes, rows, (uint32_t)cols, dy_stride, x_stride, code_of(x), stream_of(x)));
         }
         return {dx, dw, db, Tensor(), Tensor(), Tensor()};
@@ -152,6 +183,7 @@ Tensor layer_norm(const Tensor &input, const std::optional<Tensor> &weight_, con
                                   : weight.defined() ? weight.sizes()
                                   : bias.defined()   ? bias.sizes()
                                                      : input.sizes().slice(input.dim() ? input.dim() - 1 : 0);
+    check_transforms("layer_norm", {&input, &weight, &bias});
     const int64_t dims = (int64_t)shape.size();
     TORCH_CHECK_VALUE(dims > 0 && dims <= input.dim() && input.sizes().slice(input.dim() - dims) == shape, "layer_norm over ", shape,
                       " of an input of shape ", input.sizes());
@@ -178,7 +210,7 @@ Tensor embedding_forward(const Tensor &index, const Tensor &table, double scale)
     shape.push_back(table.size(1));
     Tensor y = at::empty(shape, table.options());
     if (y.numel() == 0) return y;
-    const Tensor t = table.contiguous();
+    const Tensor t = packed(table);
     check("elx_embedding_fwd", elx_embedding_fwd(index.data_ptr(), (int)index.element_size(), index.numel(), t.data_ptr(), t.size(0),
                                                  (uint32_t)t.size(1), (float)scale, y.data_ptr(), code_of(t), stream_of(t)));
     return y;
@@ -188,6 +220,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
     static Tensor forward(AutogradContext *ctx, const Tensor &index, const Tensor &table, int64_t padding, double scale) {
         ctx->save_for_backward({index});
         ctx->saved_data["table"] = at::empty({0}, table.options());    // type and device; the table itself is not kept
+        ctx->saved_data["wide"] = index.scalar_type() == at::kLong;
         ctx->saved_data["rows"] = table.size(0);
         ctx->saved_data["cols"] = table.size(1);
         ctx->saved_data["padding"] = padding;
@@ -196,23 +229,26 @@ struct Embedding : torch::autograd::Function<Embedding> {
     }
 
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        const Tensor index = ctx->get_saved_variables()[0];
+        const Tensor index = ctx->get_saved_variables()[0].contiguous();
+        const Tensor &grad = grads[0];
         const auto options = ctx->saved_data["table"].toTensor().options();
         const int64_t rows = ctx->saved_data["rows"].toInt(), cols = ctx->saved_data["cols"].toInt();
         const int64_t padding = ctx->saved_data["padding"].toInt();
         const double scale = ctx->saved_data["scale"].toDouble();
-        const c10::DeviceGuard guard(index.device());
+        const c10::DeviceGuard guard(grad.device());
+        TORCH_CHECK(cols == 0 || index.numel() == grad.numel() / cols, "embedding: a saved tensor came back in another shape");
+        check_saved("embedding", index, ctx->saved_data["wide"].toBool() ? at::kLong : at::kInt, grad.device(), index.numel());
         if (at::GradMode::is_enabled()) {    // the gradient is to be differentiated: torch's operators
             const Tensor inside = index.ge(0).logical_and(index.lt(rows));
             const Tensor table = at::zeros({rows, cols}, options).requires_grad_();
             const Tensor y = at::embedding(table, index.where(inside, at::zeros_like(index)), padding);
-            const Tensor dy = (grads[0] * scale).masked_fill(inside.logical_not().unsqueeze(-1), 0);
+            const Tensor dy = (grad * scale).masked_fill(inside.logical_not().unsqueeze(-1), 0);
             return {Tensor(), torch::autograd::grad({y}, {table}, {dy}, std::nullopt, true)[0], Tensor(), Tensor()};
         }
         Tensor dtable = at::empty({rows, cols}, options);
         const int64_t n = index.numel();
         if (n == 0 || dtable.numel() == 0) return {Tensor(), dtable.zero_(), Tensor(), Tensor()};
-        const auto [dy, stride] = rows_of(grads[0], cols);
+        const auto [dy, stride] = rows_of(grad, cols);
         const uint64_t bytes = elx_embedding_bwd_workspace(n, rows, (uint32_t)cols);
         const Tensor workspace = at::empty({(int64_t)bytes}, options.dtype(at::kByte));
         check("elx_embedding_bwd",
@@ -223,6 +259,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
 };
 
 Tensor embedding(const Tensor &input, const Tensor &weight, const std::optional<int64_t> &padding_idx, double scale) {
+    check_transforms("embedding", {&weight});
     TORCH_CHECK_VALUE(weight.dim() == 2, "embedding takes a table of two dimensions, not ", weight.dim());
     TORCH_CHECK_TYPE(input.scalar_type() == at::kLong || input.scalar_type() == at::kInt, "embedding takes int64 or int32 indices, not ",
                      c10::getDtypeNames(input.scalar_type()).first);

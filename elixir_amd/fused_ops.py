@@ -6,12 +6,13 @@ The reference swaps ``F.layer_norm`` for a third party's fused kernel (elixir/ke
 embedding to torch.  Both functions take device tensors in fp32, fp16 or bf16, compute in fp32 and round once, run on the
 current stream of the tensors' device, allocate what they return (and, in backward, a workspace) through torch's allocator,
 synchronise nothing, and can be captured into a graph.  A gradient that is itself to be differentiated
-(``create_graph=True``) is computed by torch's own operators.  What the functions cannot take they refuse; the modules fall
+(``create_graph=True``) is computed by torch's own operators; forward-mode derivatives and tracing are refused.  What the functions cannot take they refuse; the modules fall
 back to torch instead, so that a model keeps running wherever it ran."""
 from typing import Optional, Sequence, Union
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _ops_abi, _torch_ext
 
@@ -44,7 +45,7 @@ def embedding(input: torch.Tensor, weight: torch.Tensor, padding_idx: Optional[i
 
     input: int64 or int32 device tensor of any shape, up to 2^26 tokens.  weight: [rows, cols] on the same device in fp32,
         fp16 or bf16; it and the embedded tokens have up to 2^34 elements.  padding_idx: a row whose tokens add nothing to the gradient (negative: counted from the end).
-    The gradient of ``weight`` is dense, summed in fp32 in the order of the tokens (the same bits every time) and rounded
+    The gradient of ``weight`` is dense, summed in fp32 in a fixed order (the same bits every time) and rounded
     once.  The indices are not checked on the host: one outside the table gives a row of NaN and no gradient."""
     return (_ext or _load()).embedding(input, weight, padding_idx, scale)
 
@@ -53,9 +54,10 @@ def embedding(input: torch.Tensor, weight: torch.Tensor, padding_idx: Optional[i
 
 
 def _plain_eager(*tensors: Optional[torch.Tensor]) -> bool:
-    """Ordinary device tensors of a supported type, outside of autocast, of tracing and of functorch transforms: everything
-    else is torch's."""
-    if torch.compiler.is_compiling() or torch.is_autocast_enabled() or torch._C._are_functorch_transforms_active():
+    """Ordinary device tensors of a supported type, outside of autocast, of tracing and other dispatch modes, of functorch
+    transforms and of forward-mode derivatives: everything else is torch's."""
+    if (torch.compiler.is_compiling() or torch.is_autocast_enabled() or torch._C._are_functorch_transforms_active()
+            or torch.jit.is_tracing() or torch._C._len_torch_dispatch_stack() or forward_ad._current_level >= 0):
         return False
     for t in tensors:
         if t is not None and not (type(t) in (torch.Tensor, nn.Parameter) and t.is_cuda and t.layout == torch.strided):
@@ -65,7 +67,8 @@ def _plain_eager(*tensors: Optional[torch.Tensor]) -> bool:
 
 class FusedLayerNorm(nn.LayerNorm):
     """``nn.LayerNorm`` on ``layer_norm``.  Same parameters, same state; inputs that function does not take (other types or
-    devices, more than 16,384 elements per row, autocast, compiled or transformed code) go to torch."""
+    devices, more than 16,384 elements per row, autocast, compiled, traced or transformed code, forward-mode derivatives) go
+    to torch."""
 
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         w, b = self.weight, self.bias
@@ -82,8 +85,8 @@ class FusedLayerNorm(nn.LayerNorm):
 
 class FusedEmbedding(nn.Embedding):
     """``nn.Embedding`` on ``embedding``, with a factor on the embedded rows (``scale``).  Same parameters, same state;
-    ``max_norm``, ``scale_grad_by_freq`` and ``sparse``, other types or devices, autocast, compiled or transformed code go to
-    torch (and are scaled after it)."""
+    ``max_norm``, ``scale_grad_by_freq`` and ``sparse``, other types or devices, autocast, compiled, traced or transformed
+    code and forward-mode derivatives go to torch (and are scaled after it)."""
 
     scale: float = 1.0    # also that of a module which was an nn.Embedding before
 

@@ -5,6 +5,7 @@ import pickle
 import pytest
 import torch
 from torch import nn
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import elixir_amd as ea
 from elixir_amd import _abi, _ops_abi, _torch_ext
@@ -149,3 +150,20 @@ def test_scale_of_the_embedding_module():
     assert torch.equal(emb(torch.tensor([3])), emb.weight[3:4] * 2)
     emb = ea.FusedEmbedding(10, 4, max_norm=0.1)
     assert emb(torch.tensor([3])).norm() <= 0.1001
+
+
+def test_transforms_that_see_only_the_allocations_are_refused():
+    """A tangent must not be dropped and a trace must not record an empty tensor in place of the result."""
+    x, w, index = torch.randn(3, 8), torch.randn(8), torch.tensor([1, 2])
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError, match='forward-mode'):
+            ea.layer_norm(dual, w)
+        with pytest.raises(NotImplementedError, match='forward-mode'):
+            ea.layer_norm(x, torch.autograd.forward_ad.make_dual(w, w))
+        with pytest.raises(NotImplementedError, match='forward-mode'):
+            ea.embedding(index, dual)
+    for call in (lambda: torch.jit.trace(lambda t: ea.layer_norm(t, w), x, check_trace=False),
+                 lambda: make_fx(lambda t: ea.layer_norm(t, w))(x), lambda: make_fx(lambda t: ea.embedding(index, t))(x)):
+        with pytest.raises(NotImplementedError, match='traced'):
+            call()

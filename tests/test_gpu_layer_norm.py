@@ -357,3 +357,50 @@ def test_the_module_runs_the_kernel_and_falls_back(monkeypatch):
     with pytest.raises(RuntimeError):
         norm(x[:, :40])
     assert calls == [1]
+
+
+def test_hooks_that_hand_back_another_tensor_are_refused():
+    """The backward launch reads what the hooks of the saved tensors return: another type, size or device is an error."""
+    def loss(unpack):
+        leaves = [t.requires_grad_() for t in inputs(40, 96, torch.float32)[:3]]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            return ea.layer_norm(*leaves).sum()
+
+    for unpack in (lambda t: t.half(), lambda t: t.cpu(), lambda t: t[:1].clone(), lambda t: t.t() if t.dim() == 2 and len(t) == 40 else t):
+        with pytest.raises(RuntimeError, match='came back'):
+            loss(unpack).backward()
+    loss(lambda t: t.t().contiguous().t() if t.dim() == 2 else t).backward()    # another layout is fine
+
+
+def test_negated_views():
+    """A view that negates what lies in memory (the imaginary part of a conjugate) is read as what it stands for."""
+    z = torch.randn(6, 1, 33, dtype=torch.complex64, device=DEV).conj()
+    x = z.imag.transpose(0, 1)[0]
+    assert x.is_neg()
+    w = torch.randn(33, device=DEV)
+    lazy = torch._neg_view(x.neg().contiguous())
+    for t in (x, lazy):
+        want = ea.layer_norm(x.clone().contiguous().resolve_neg(), w)
+        assert torch.equal(ea.layer_norm(t, w), want)
+    assert torch.equal(ea.layer_norm(x.resolve_neg(), torch._neg_view(w.neg())), ea.layer_norm(x.resolve_neg(), w))
+
+
+def test_transforms_go_to_torch_or_are_refused():
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, b, _ = (t.detach() for t in inputs(5, 48, torch.float32))
+    norm = ea.FusedLayerNorm(48).to(DEV).requires_grad_(False)
+    plain = torch.nn.LayerNorm(48).to(DEV).requires_grad_(False)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, b.expand(5, 48).contiguous())
+        got, want = forward_ad.unpack_dual(norm(dual)), forward_ad.unpack_dual(plain(dual))
+        assert torch.equal(got.tangent, want.tangent) and torch.equal(got.primal, want.primal)
+        with pytest.raises(NotImplementedError):
+            ea.layer_norm(dual, w, b)
+    for traced in (make_fx(lambda t: norm(t))(x), torch.jit.trace(norm, x, check_trace=False)):
+        other = torch.randn(5, 48, device=DEV)
+        assert torch.equal(traced(other), plain(other))
+    for call in (lambda: torch.func.vmap(lambda t: ea.layer_norm(t, w, b))(x.view(5, 1, 48)),
+                 lambda: torch.func.grad(lambda t: ea.layer_norm(x, t, b).sum())(w)):
+        with pytest.raises(RuntimeError):
+            call()
