@@ -8,10 +8,10 @@
 // have them side by side the tokens are sorted by index: a stable radix sort of (index, position), least significant digit
 // first -- in LDS by one workgroup where the tokens fit there, else by up to 64 workgroups, one launch per digit and one to
 // begin with.  Then
-//   sum_kernel   one workgroup per tile of 8 or 24 sorted tokens: a run of equal indices inside the tile goes straight to its
+//   sum_kernel   a workgroup per tile of 8 or 24 sorted tokens: a run of equal indices inside the tile goes straight to its
 //                row, a run that reaches over an end of the tile leaves an fp32 partial row; the workgroups behind these
 //                clear the rows that no token names, which a search in the sorted tokens tells them: dW is written once;
-//   join_kernel  adds up the partial rows of the runs over several tiles (a frequent token), in the order of the tiles.
+//   join_kernel  adds up the partial rows of the runs over several tiles (a frequent token), in a fixed order.
 // No atomics on values: the result is the same every time, and a token that fills the batch is summed by many workgroups.
 // (Clearing dW beside the sort instead, in the idle workgroups of its launches, made the sort three times slower -- its
 // chain of small reads waits behind the stores -- and wrote the touched rows twice: 89 us against 70 for 16384 tokens in a
@@ -97,8 +97,12 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / kWave;
 constexpr uint32_t kMaxBins = 1024;       // ten bits per pass
 constexpr uint32_t kMaxSortBlocks = 64;
-constexpr uint32_t kSmallTokens = 4096;    // sorted by one workgroup
-constexpr uint32_t kGathered = 8192;       // counters of the next pass that a workgroup gathers in LDS
+// Up to that many tokens are sorted by one workgroup in one launch (768 columns: 1021 tokens 26 us with it, 29.5 in several
+// launches; 2048 tokens 30.1 and 31.2; 4096 tokens 38.4 and 33.5).
+constexpr uint32_t kSmallTokens = 2048;
+// Counters of the next pass that a workgroup gathers in LDS.  Added to memory one by one they cost a pass of 16384 tokens 15 us
+// instead of 6: frequent tokens meet in one word.
+constexpr uint32_t kGathered = 16384;
 
 struct Keys {
     const void *index;    // first pass: the indices themselves (keys == nullptr)
@@ -169,11 +173,13 @@ __global__ __launch_bounds__(kSortThreads) void scatter_kernel(Keys in, uint64_t
                                                                uint32_t *__restrict__ clear, uint32_t *__restrict__ keys_out,
                                                                uint32_t *__restrict__ positions_out) {
     const uint32_t bins = 1u << bits;
-    __shared__ uint32_t base[kMaxBins];
-    __shared__ uint16_t in_wave[kSortWaves][kMaxBins];
+    __shared__ uint32_t base[2][kMaxBins];
+    __shared__ uint16_t in_wave[2][kSortWaves][kMaxBins];
     __shared__ uint32_t wave_total[kSortWaves];
     __shared__ uint32_t gathered[kGathered];
     const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const uint64_t begin = (uint64_t)blockIdx.x * per_block + threadIdx.x;
+    uint32_t key = begin < n ? key_at(in, begin) : 0;
 
     // one digit per thread: all its tokens, and those in earlier blocks
     uint32_t total = 0, before = 0;
@@ -189,34 +195,46 @@ __global__ __launch_bounds__(kSortThreads) void scatter_kernel(Keys in, uint64_t
             }
         }
 #pragma unroll
-        for (int w = 0; w < kSortWaves; ++w) in_wave[w][threadIdx.x] = 0;
+        for (int w = 0; w < kSortWaves; ++w) in_wave[0][w][threadIdx.x] = 0;
         if (clear) clear[blockIdx.x * bins + threadIdx.x] = 0;
     }
-    const uint32_t smaller = digits_before(total, wave_total);
-    if (threadIdx.x < bins) base[threadIdx.x] = smaller + before;
+    uint32_t place = digits_before(total, wave_total) + before;    // of the next token with this thread's digit
     // where they fit, the next pass's counts are gathered in LDS: a frequent token would have a thousand threads add to one
     // word of memory
     const uint32_t counters = next ? gridDim.x * bins : 0;
     const bool gather = counters <= kGathered;
     if (gather)
         for (uint32_t d = threadIdx.x; d < counters; d += kSortThreads) gathered[d] = 0;
-    __syncthreads();
 
-    const uint64_t begin = (uint64_t)blockIdx.x * per_block;
-    for (uint32_t round = 0; round < per_block; round += kSortThreads) {
-        const uint64_t i = begin + round + threadIdx.x;
+    // two barriers a round: the tables of a round are those of the round before the last, which everybody has left
+    for (uint32_t round = 0, turn = 0; round < per_block; round += kSortThreads, turn ^= 1) {
+        const uint64_t i = begin + round;
         const bool live = i < n;
-        const uint32_t key = live ? key_at(in, i) : 0;
+        const uint32_t position = !live ? 0 : in.keys ? in.positions[i] : (uint32_t)i;
         const uint32_t digit = (key >> shift) & (bins - 1);
         const uint64_t same = lanes_with(digit, bits, live);
         const uint32_t rank = __builtin_popcountll(same & ((1ull << lane) - 1));
-        if (live && rank == 0) in_wave[wave][digit] = (uint16_t)__builtin_popcountll(same);
+        if (live && rank == 0) in_wave[turn][wave][digit] = (uint16_t)__builtin_popcountll(same);
+        const bool more = round + kSortThreads < per_block && i + kSortThreads < n;
+        const uint32_t next_key = more ? key_at(in, i + kSortThreads) : 0;    // on its way
+        __syncthreads();
+        if (threadIdx.x < bins) {    // counts become places
+            base[turn][threadIdx.x] = place;
+            uint32_t c = 0;
+#pragma unroll
+            for (int w = 0; w < kSortWaves; ++w) {
+                const uint32_t of_wave = in_wave[turn][w][threadIdx.x];
+                in_wave[turn][w][threadIdx.x] = (uint16_t)c;
+                in_wave[turn ^ 1][w][threadIdx.x] = 0;
+                c += of_wave;
+            }
+            place += c;
+        }
         __syncthreads();
         if (live) {
-            uint32_t at = base[digit] + rank;
-            for (uint32_t w = 0; w < wave; ++w) at += in_wave[w][digit];
+            const uint32_t at = base[turn][digit] + in_wave[turn][wave][digit] + rank;
             keys_out[at] = key;
-            positions_out[at] = in.keys ? in.positions[i] : (uint32_t)i;
+            positions_out[at] = position;
             if (next) {
                 const uint32_t slot = at / per_block * bins + ((key >> (shift + bits)) & (bins - 1));
                 if (gather)
@@ -225,21 +243,12 @@ __global__ __launch_bounds__(kSortThreads) void scatter_kernel(Keys in, uint64_t
                     atomicAdd(&next[slot], 1u);
             }
         }
-        __syncthreads();
-        if (threadIdx.x < bins) {    // the round's tokens become earlier ones
-            uint32_t c = 0;
-#pragma unroll
-            for (int w = 0; w < kSortWaves; ++w) {
-                c += in_wave[w][threadIdx.x];
-                in_wave[w][threadIdx.x] = 0;
-            }
-            base[threadIdx.x] += c;
-        }
-        __syncthreads();
+        key = next_key;
     }
-    if (gather)
-        for (uint32_t d = threadIdx.x; d < counters; d += kSortThreads)
-            if (gathered[d]) atomicAdd(&next[d], gathered[d]);
+    if (!gather || !next) return;
+    __syncthreads();
+    for (uint32_t d = threadIdx.x; d < counters; d += kSortThreads)
+        if (gathered[d]) atomicAdd(&next[d], gathered[d]);
 }
 
 // The whole sort of up to kSmallTokens tokens by one workgroup, the same steps in LDS.
@@ -310,16 +319,22 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(Keys in, uint3
 // sums
 // ---------------------------------------------------------------------------------------------
 
-// Tokens of a tile.  Few tokens: short tiles, the launch lasts as long as its longest chain of them (1021 tokens of a
-// 50257 x 768 fp16 table: 25 us with 8, 29 with 16, 33 with 24).  Many: long ones, every end of a tile that cuts a run costs
-// two fp32 rows (16384 tokens of 50272 x 2048 bf16: 68 us with 24, 71 with 16, 76 with 8; 75 with 32, whose rows take too
-// many registers).
+// Tokens of a tile.  Few elements: short tiles, the launch lasts as long as its longest chain of them (768 columns of fp16:
+// 1021 tokens 25 us with 8, 33 with 24; 8192 tokens 38 and 46; 16384 tokens 42 and 45).  Many: long ones, every end of a tile
+// that cuts a run costs two fp32 rows (16384 x 2048 bf16: 74 us with 8, 69 with 24, 75 with 32, whose rows take too many
+// registers; 8192 x 4096 fp32: 147 with 8, 136 with 24).
 constexpr uint32_t kTileFew = 8, kTileMany = 24;
-constexpr uint32_t kFewTokens = kSmallTokens;
-constexpr int kSumThreads = 256;
+constexpr uint64_t kFewElems = 1ull << 24;
+constexpr int kSumThreads = 256;    // at most
 
-constexpr uint32_t kFillBytes = 16u << 10;    // cleared by one workgroup, about
-constexpr uint32_t kFillRows = 2048;          // rows of a clearing workgroup, at most
+// A thread of a clearing workgroup clears about that much: with more, the last workgroups run on alone (8192 tokens in
+// 32000 x 4096 fp32: 135 us with 64 bytes, 145 with 128, 150 with 256), with less the search weighs more (16384 x 2048
+// bf16: 69 us with 64, 83 with 32).
+constexpr uint32_t kFillBytes = 64;
+constexpr uint32_t kFillRows = 2048;      // rows of a clearing workgroup, at most
+// It looks at that many tokens of its rows one by one; beyond, a search per row is shorter (16384 tokens of a table of 30 rows:
+// 21 us; 69 us when all are looked at).
+constexpr uint32_t kScanTokens = 1024;
 
 // First place in keys[0, n) whose key is at least `key`: the wavefront looks at 64 places at a time.
 __device__ __forceinline__ uint32_t first_at_least(const uint32_t *__restrict__ keys, uint32_t n, uint32_t key) {
@@ -339,32 +354,50 @@ __device__ __forceinline__ uint32_t first_at_least(const uint32_t *__restrict__ 
     return lo;
 }
 
-// First place in keys[from, n) whose key is not `key` (all before it are).
-__device__ __forceinline__ uint32_t key_run_end(const uint32_t *__restrict__ keys, uint32_t n, uint32_t from, uint32_t key) {
-    return from >= n ? n : from + first_at_least(keys + from, n - from, key + 1);
+// Whether keys[lo, hi) names `key`; the thread by itself.
+__device__ __forceinline__ bool names(const uint32_t *__restrict__ keys, uint32_t lo, uint32_t hi, uint32_t key) {
+    const uint32_t end = hi;
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (keys[mid] < key)
+            lo = mid + 1;
+        else
+            hi = mid;
+    }
+    return lo < end && keys[lo] == key;
 }
 
 // Clears those of the rows [row, row + count) that no token names.  A row is cleared in units of `unit` bytes.
 __device__ __forceinline__ void clear_rows(const uint32_t *__restrict__ keys, uint32_t n, uint32_t row, uint32_t count, char *base,
                                            uint32_t row_bytes, uint32_t unit) {
     __shared__ uint32_t named[kFillRows / 32];
-    for (uint32_t i = threadIdx.x; i < kFillRows / 32; i += kSumThreads) named[i] = 0;
+    __shared__ uint32_t bounds[2];
+    const uint32_t threads = blockDim.x, wave = threadIdx.x / kWave, waves = threads / kWave;
+    for (uint32_t i = threadIdx.x; i < kFillRows / 32; i += threads) named[i] = 0;
+    // the tokens of these rows are keys[lo, hi): its ends by two wavefronts side by side
+    if (wave == 0) {
+        const uint32_t at = first_at_least(keys, n, row);
+        if (threadIdx.x == 0) bounds[0] = at;
+    }
+    if (wave == waves - 1) {
+        const uint32_t at = first_at_least(keys, n, row + count);
+        if (threadIdx.x % kWave == 0) bounds[1] = at;
+    }
     __syncthreads();
-    if (threadIdx.x < kWave) {
-        uint32_t at = first_at_least(keys, n, row);
-        while (at < n) {
-            const uint32_t key = at + threadIdx.x < n ? keys[at + threadIdx.x] : ~0u;
-            if (key < row + count) atomicOr(&named[(key - row) / 32], 1u << ((key - row) % 32));
-            const uint32_t top = (uint32_t)__builtin_amdgcn_readlane((int)key, kWave - 1);
-            if (top >= row + count) break;
-            // behind this key's run: the 64 places looked at may all be of it, and so may thousands more
-            at = key_run_end(keys, n, at + kWave, top);
+    const uint32_t lo = bounds[0], hi = bounds[1];
+    if (hi - lo <= kScanTokens) {    // few: look at each
+        for (uint32_t i = lo + threadIdx.x; i < hi; i += threads) {
+            const uint32_t key = keys[i] - row;
+            atomicOr(&named[key / 32], 1u << (key % 32));
         }
+    } else {    // frequent tokens: look for each row
+        for (uint32_t r = threadIdx.x; r < count; r += threads)
+            if (names(keys, lo, hi, row + r)) atomicOr(&named[r / 32], 1u << (r % 32));
     }
     __syncthreads();
     const uint32_t units = row_bytes / unit;
     uint32_t r = threadIdx.x / units, u = threadIdx.x % units;
-    const uint32_t rows_per_turn = kSumThreads / units, units_per_turn = kSumThreads % units;
+    const uint32_t rows_per_turn = threads / units, units_per_turn = threads % units;
     while (r < count) {
         if (!(named[r / 32] >> (r % 32) & 1)) {
             char *to = base + (uint64_t)(row + r) * row_bytes + (uint64_t)u * unit;
@@ -413,7 +446,7 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const uint32_t *__rest
     }
     const uint32_t tile = blockIdx.x / clear.chunks;
     const uint32_t first = tile * kTokens;
-    const uint32_t c = (blockIdx.x % clear.chunks * kSumThreads + threadIdx.x) * V;
+    const uint32_t c = (blockIdx.x % clear.chunks * blockDim.x + threadIdx.x) * V;
     const bool mine = c < cols;
     // the tile's tokens, one per lane: from here on they are read from registers
     const uint32_t lane = threadIdx.x % kWave;
@@ -468,52 +501,92 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const uint32_t *__rest
 }
 
 constexpr int kJoinThreads = 1024;
+constexpr uint32_t kJoinLanes = 16, kJoinGroups = kJoinThreads / kJoinLanes;
+constexpr uint32_t kJoinAlone = 8;
+static_assert(kJoinGroups == kWave, "a wavefront looks at the tiles of all groups");
 
-// One workgroup per tile whose last run starts there and goes on; `lanes` threads side by side over the columns (J each),
-// the groups of lanes take the run's tiles in turn, and the groups are added up in their order.
+// Rows of runs over several tiles.  A workgroup looks at 64 tiles and at 16 J columns.  A group of 16 lanes per tile whose last
+// run starts there and goes on adds its partial rows up; a run over more than kJoinAlone further tiles is left to the whole
+// workgroup: its groups take the run's tiles in turn and are added up in their order.  Narrow slices of the columns let many
+// workgroups share the run of a token that fills the batch (16384 x 2048 bf16 of one token: 35 us in all, 124 with the
+// whole row in one workgroup per run).
 template <int D, int J>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(const uint32_t *__restrict__ keys, uint32_t n, uint32_t vocab, uint32_t cols,
                                                             float scale, typename Elem<D>::scalar *__restrict__ dtable,
-                                                            const float *__restrict__ partials, uint32_t lanes, uint32_t tokens) {
-    const uint32_t first = blockIdx.x * tokens, next = first + tokens;
-    if (next >= n) return;
-    const uint32_t key = keys[next - 1], behind = keys[next], before = first ? keys[first - 1] : ~0u;
-    const uint32_t further = next + tokens < n ? keys[next + tokens] : ~0u;    // asked for together
-    if (key >= vocab || behind != key || before == key) return;    // ends here, or came in from the tile before
-    // the run reaches tile `lo`; find the last that it reaches
-    uint32_t lo = blockIdx.x + 1, hi = further == key ? (n + tokens - 1) / tokens - 1 : lo;
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi + 1) / 2;
-        if (keys[mid * tokens] == key)
-            lo = mid;
-        else
-            hi = mid - 1;
-    }
-    __shared__ float sums[J][kJoinThreads];
-    const uint32_t group = threadIdx.x / lanes, groups = kJoinThreads / lanes, lane = threadIdx.x % lanes;
-    for (uint32_t c0 = 0; c0 < cols; c0 += lanes * J) {
-        const uint32_t c = c0 + lane * J;
-        float s[J] = {};
-        if (c < cols) {
-            auto add = [&](uint64_t slot) {
-                float x[J];
-                __builtin_memcpy(x, __builtin_assume_aligned(partials + slot * cols + c, J * 4), J * 4);
+                                                            const float *__restrict__ partials, uint32_t tokens, uint32_t chunks) {
+    __shared__ uint32_t run_key[kJoinGroups], run_last[kJoinGroups];    // of the run that each tile begins: its key, its last tile
+    __shared__ uint64_t long_runs;                                      // the tiles whose run is left to the workgroup
+    __shared__ float sums[kJoinGroups][kJoinLanes * J];
+    const uint32_t tile0 = blockIdx.x / chunks * kJoinGroups, c0 = blockIdx.x % chunks * (kJoinLanes * J);
+    if (threadIdx.x < kWave) {
+        const uint32_t tile = tile0 + threadIdx.x, next = (tile + 1) * tokens;
+        uint32_t key = ~0u, last = 0;
+        if (next < n) {
+            // the tile's last key, the one before it and the first ones of the tiles behind it, asked for together
+            const uint32_t k = keys[next - 1], before = tile ? keys[tile * tokens - 1] : ~0u;
+            uint32_t ahead[kJoinAlone + 1];
 #pragma unroll
-                for (int j = 0; j < J; ++j) s[j] += x[j];
-            };
-            if (group == 0) add((uint64_t)blockIdx.x * 2 + 1);
-#pragma unroll 4
-            for (uint32_t t = blockIdx.x + 1 + group; t <= lo; t += groups) add((uint64_t)t * 2);
+            for (uint32_t i = 0; i <= kJoinAlone; ++i) {
+                const uint32_t at = next + i * tokens;
+                ahead[i] = at < n ? keys[at] : ~0u;
+            }
+            uint32_t reach = 0;    // tiles behind this one that start with the key: keys are sorted, so they come first
+#pragma unroll
+            for (uint32_t i = 0; i <= kJoinAlone; ++i) reach += ahead[i] == k ? 1 : 0;
+            if (k < vocab && before != k && reach) {
+                key = k;
+                last = tile + reach;
+                uint32_t hi = reach > kJoinAlone ? (n + tokens - 1) / tokens - 1 : last;    // beyond what has been looked at
+                while (last < hi) {
+                    const uint32_t mid = (last + hi + 1) / 2;
+                    if (keys[mid * tokens] == k)
+                        last = mid;
+                    else
+                        hi = mid - 1;
+                }
+            }
         }
+        run_key[threadIdx.x] = key;
+        run_last[threadIdx.x] = last;
+        const uint64_t far = __builtin_amdgcn_ballot_w64(key != ~0u && last - tile > kJoinAlone);
+        if (threadIdx.x == 0) long_runs = far;
+    }
+    __syncthreads();
+    const uint32_t group = threadIdx.x / kJoinLanes, lane = threadIdx.x % kJoinLanes, c = c0 + lane * J;
+    const bool mine = c < cols;
+    auto add = [&](uint64_t slot, float (&s)[J]) {
+        float x[J];
+        __builtin_memcpy(x, __builtin_assume_aligned(partials + slot * cols + c, J * 4), J * 4);
 #pragma unroll
-        for (int j = 0; j < J; ++j) sums[j][threadIdx.x] = s[j];
-        __syncthreads();
-        if (group == 0 && c < cols) {
-            for (uint32_t g = 1; g < groups; ++g)
-#pragma unroll
-                for (int j = 0; j < J; ++j) s[j] += sums[j][g * lanes + lane];
+        for (int j = 0; j < J; ++j) s[j] += x[j];
+    };
+    {
+        const uint32_t key = run_key[group], tile = tile0 + group, last = run_last[group];
+        if (mine && key != ~0u && last - tile <= kJoinAlone) {
+            float s[J] = {};
+            add((uint64_t)tile * 2 + 1, s);
+#pragma unroll 4
+            for (uint32_t t = tile + 1; t <= last; ++t) add((uint64_t)t * 2, s);
 #pragma unroll
             for (int j = 0; j < J; ++j) dtable[(uint64_t)key * cols + c + j] = Elem<D>::from_f32(s[j] * scale);
+        }
+    }
+    for (uint64_t left = long_runs; left; left &= left - 1) {
+        const uint32_t g = __builtin_ctzll(left), key = run_key[g], tile = tile0 + g, last = run_last[g];
+        float s[J] = {};
+        if (mine) {
+            if (group == 0) add((uint64_t)tile * 2 + 1, s);
+#pragma unroll 8
+            for (uint32_t t = tile + 1 + group; t <= last; t += kJoinGroups) add((uint64_t)t * 2, s);
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) sums[group][lane * J + j] = s[j];
+        __syncthreads();
+        if (threadIdx.x < kJoinLanes * J && c0 + threadIdx.x < cols) {
+            float all = 0.0f;
+#pragma unroll 16
+            for (uint32_t i = 0; i < kJoinGroups; ++i) all += sums[i][threadIdx.x];
+            dtable[(uint64_t)key * cols + c0 + threadIdx.x] = Elem<D>::from_f32(all * scale);
         }
         __syncthreads();
     }
@@ -550,18 +623,21 @@ struct Shape {
     int passes, bits;
 };
 
-Shape shape_of(uint64_t n, uint64_t vocab) {
+Shape shape_of(uint64_t n, uint64_t vocab, uint32_t cols) {
     Shape s;
-    // rounds of 1024 tokens per sorting workgroup, so many that at most kMaxSortBlocks of them share the work
-    const uint64_t rounds = (n + (uint64_t)kSortThreads * kMaxSortBlocks - 1) / ((uint64_t)kSortThreads * kMaxSortBlocks);
-    s.per_block = (uint32_t)(rounds * kSortThreads);
-    s.sort_blocks = (uint32_t)((n + s.per_block - 1) / s.per_block);
-    s.tokens = n <= kFewTokens ? kTileFew : kTileMany;
-    s.tiles = (uint32_t)((n + s.tokens - 1) / s.tokens);
     int all = 1;    // keys are 0 .. vocab
     while (all < 32 && (vocab >> all)) ++all;
     s.passes = (all + 9) / 10;
     s.bits = (all + s.passes - 1) / s.passes;
+    // Rounds of 1024 tokens per sorting workgroup, so many that at most kMaxSortBlocks of them share the work -- half of them
+    // where their counters of the next pass then fit LDS (131072 tokens of 128256 rows: 97 us with half, 108 with all; a
+    // quarter costs more than it gains, 1000000 rows: 140 us, 124 with all).
+    const uint64_t most = s.passes > 1 && (kMaxSortBlocks << s.bits) == 2 * kGathered ? kMaxSortBlocks / 2 : kMaxSortBlocks;
+    const uint64_t rounds = (n + kSortThreads * most - 1) / (kSortThreads * most);
+    s.per_block = (uint32_t)(rounds * kSortThreads);
+    s.sort_blocks = (uint32_t)((n + s.per_block - 1) / s.per_block);
+    s.tokens = n * cols <= kFewElems ? kTileFew : kTileMany;
+    s.tiles = (uint32_t)((n + s.tokens - 1) / s.tokens);
     return s;
 }
 
@@ -572,26 +648,29 @@ int launch_sums(const Shape &s, const uint32_t *keys, const uint32_t *positions,
                 uint64_t dy_stride, uint32_t cols, float scale, void *dtable, float *partials, hipStream_t stream) {
     typedef typename Elem<D>::scalar T;
     Clear clear;
-    clear.chunks = ((cols + V - 1) / V + kSumThreads - 1) / kSumThreads;
+    const uint32_t accesses = (cols + V - 1) / V;
+    clear.chunks = (accesses + kSumThreads - 1) / kSumThreads;
+    // whole wavefronts, no more than the columns need: idle ones would take the place of other tiles
+    const dim3 threads(((accesses + clear.chunks - 1) / clear.chunks + kWave - 1) / kWave * kWave);
     clear.tile_blocks = s.tiles * clear.chunks;
     clear.row_bytes = cols * (uint32_t)sizeof(T);
     clear.unit = clear.row_bytes % 16 == 0 && aligned16(dtable) ? 16 : (uint32_t)sizeof(T);
-    const uint32_t rows = kFillBytes / clear.row_bytes;
+    const uint32_t rows = kFillBytes * threads.x / clear.row_bytes;
     clear.rows_per_block = rows < 1 ? 1 : rows > kFillRows ? kFillRows : rows;
     const uint64_t clear_blocks = (vocab + clear.rows_per_block - 1) / clear.rows_per_block;
     const dim3 grid((uint32_t)(clear.tile_blocks + clear_blocks));
     if (s.tokens == kTileFew)
-        hipLaunchKernelGGL((sum_kernel<D, V, kTileFew>), grid, dim3(kSumThreads), 0, stream, keys, positions, (uint32_t)n, (uint32_t)vocab,
+        hipLaunchKernelGGL((sum_kernel<D, V, kTileFew>), grid, threads, 0, stream, keys, positions, (uint32_t)n, (uint32_t)vocab,
                            (const T *)dy, dy_stride, cols, scale, (T *)dtable, partials, clear);
     else
-        hipLaunchKernelGGL((sum_kernel<D, V, kTileMany>), grid, dim3(kSumThreads), 0, stream, keys, positions, (uint32_t)n,
+        hipLaunchKernelGGL((sum_kernel<D, V, kTileMany>), grid, threads, 0, stream, keys, positions, (uint32_t)n,
                            (uint32_t)vocab, (const T *)dy, dy_stride, cols, scale, (T *)dtable, partials, clear);
     if (int rc = (int)hipGetLastError()) return rc;
     if (s.tiles < 2) return 0;
     constexpr int J = V > 1 ? 4 : 1;
-    const uint32_t lanes = lanes_for((cols + J - 1) / J, 256);
-    hipLaunchKernelGGL((join_kernel<D, J>), dim3(s.tiles - 1), dim3(kJoinThreads), 0, stream, keys, (uint32_t)n, (uint32_t)vocab, cols,
-                       scale, (T *)dtable, partials, lanes, s.tokens);
+    const uint32_t chunks = (cols + kJoinLanes * J - 1) / (kJoinLanes * J);
+    hipLaunchKernelGGL((join_kernel<D, J>), dim3((s.tiles - 1 + kJoinGroups - 1) / kJoinGroups * chunks), dim3(kJoinThreads), 0, stream, keys,
+                       (uint32_t)n, (uint32_t)vocab, cols, scale, (T *)dtable, partials, s.tokens, chunks);
     return (int)hipGetLastError();
 }
 
@@ -627,7 +706,7 @@ int elx_embedding_fwd(const void *index, int index_bytes, uint64_t n, const void
 
 uint64_t elx_embedding_bwd_workspace(uint64_t n, uint64_t vocab, uint32_t cols) {
     if (n == 0 || n > kMaxTokens || vocab == 0 || vocab > kMaxVocab || cols == 0 || cols > kMaxCols || n * cols > kMaxElems) return 0;
-    const Shape s = shape_of(n, vocab);
+    const Shape s = shape_of(n, vocab, cols);
     return 4 * round256(4 * n) + 3 * round256((uint64_t)s.sort_blocks * kMaxBins * 4) + round256((uint64_t)s.tiles * 2 * cols * 4);
 }
 
@@ -642,7 +721,7 @@ int elx_embedding_bwd(const void *index, int index_bytes, uint64_t n, const void
     const uint32_t es = elem_size(dtype), v = 16 / es;
     if (((uintptr_t)index & (index_bytes - 1)) || (((uintptr_t)dy | (uintptr_t)dtable) & (es - 1)) || ((uintptr_t)workspace & 15u))
         return ELX_E_ALIGN;
-    const Shape s = shape_of(n, vocab);
+    const Shape s = shape_of(n, vocab, cols);
     char *at = (char *)workspace;
     uint32_t *keys[2], *positions[2];
     for (int i = 0; i < 2; ++i) {

@@ -5,7 +5,8 @@
 //   dx = rstd * (t - mean(t) - h * mean(t * h)),   dw = sum over rows of dy * h,   db = sum over rows of dy
 //
 // A row is held in registers from its one read to its one write: W wavefronts per row, N accesses of V elements per lane.
-// Short rows (a norm over the heads of attention) share a wavefront: L lanes per row, 64 / L rows.
+// Short rows (a norm over the heads of attention) share a wavefront: L lanes per row, 64 / L rows (262144 x 64 bf16: 13 us
+// forward and 23 us backward, against 62 and 93 with a wavefront per row).
 // The variance is taken from the centred values in a second pass over the registers, so a large mean costs no digits.  All
 // sums are in fp32 (per lane, then inside the wavefront, then over wavefronts through LDS), the one rounding to the
 // tensor's type is at the store.
@@ -14,6 +15,10 @@
 // db of its own columns in registers over all its rows.  The row groups of a workgroup are added up in LDS, one partial row
 // per workgroup goes to a workspace, and a second launch adds the partial rows up in a fixed order: no atomics, the same
 // result every time.
+//
+// Both passes are bound by HBM where rows are many: 16384 x 4096 fp32 takes 93 us forward and 116 us backward from memory
+// (0.54 and 0.81 GB: 5.8 and 6.9 TB/s; 77 us forward where the cache holds a part), 8192 x 2048 bf16 12.3 and 19.6 us, where
+// the start and the end of a launch show.  A single row takes 2 us forward.  dw and db cost a second launch of 4 to 5 us.
 #include "elx_ops_device.h"
 
 using namespace elx_ops;
@@ -437,21 +442,28 @@ int launch_fwd(const Fwd &a) {
     return (int)hipGetLastError();
 }
 
-// accesses per lane for `per_wave` accesses of a row per wavefront, rounded up to what is compiled
+// wavefronts per row and accesses per lane, the latter rounded up to what is compiled
 template <int D, int V>
 int dispatch_fwd(const Fwd &a) {
     const uint32_t accesses = (a.cols + kWave * V - 1) / (kWave * V);    // wavefront-wide accesses of a row
-    constexpr uint32_t most = 64 / V;                                    // 64 elements per lane
-    // four wavefronts read a row in a quarter of the steps: for long rows, and where there are few
-    if (accesses > most || accesses >= 8 || (a.rows < 4096 && accesses >= 4)) {
+    // Four wavefronts read a long row in a quarter of the steps, one wavefront needs no barrier:
+    //   16384 x 4096 fp32   77 us with four, 93 with one      32768 x 2048 bf16   46 us with four, 42 with one
+    //   32768 x 4096 bf16   79              100                8192 x 2048 bf16   14              10.6
+    //    8191 x 1025 fp16   18               25                8191 x 1023 fp16   13.9            12.6
+    // With few rows it is the steps that count (1024 x 2048 bf16: 4.5 us with four, 5.5 with one; 4096 x 2048: 7.1, 6.8).
+    if (accesses >= (V == 1 ? 17 : 8) || (a.rows < 4096 && accesses >= 4)) {
         const uint32_t n = (accesses + 3) / 4;
         if (n <= 1) return launch_fwd<D, V, 1, 4>(a);
         if (n <= 2) return launch_fwd<D, V, 2, 4>(a);
         if (n <= 4) return launch_fwd<D, V, 4, 4>(a);
+        if (n <= 8) return launch_fwd<D, V, 8, 4>(a);
         if constexpr (V <= 4)
             if (n <= 16) return launch_fwd<D, V, 16, 4>(a);
-        if constexpr (V == 1) return launch_fwd<D, V, 64, 4>(a);
-        if constexpr (V > 1) return launch_fwd<D, V, most, 4>(a);
+        if constexpr (V == 1) {
+            if (n <= 32) return launch_fwd<D, V, 32, 4>(a);
+            if (n <= 64) return launch_fwd<D, V, 64, 4>(a);
+        }
+        return ELX_E_SIZE;
     }
     if (a.cols <= 4 * V) return launch_fwd<D, V, 1, 1, 4>(a);
     if (a.cols <= 8 * V) return launch_fwd<D, V, 1, 1, 8>(a);
@@ -461,9 +473,8 @@ int dispatch_fwd(const Fwd &a) {
     if (accesses <= 2) return launch_fwd<D, V, 2, 1>(a);
     if (accesses <= 4) return launch_fwd<D, V, 4, 1>(a);
     if (accesses <= 8) return launch_fwd<D, V, 8, 1>(a);
-    if constexpr (V <= 4)
+    if constexpr (V == 1)
         if (accesses <= 16) return launch_fwd<D, V, 16, 1>(a);
-    if constexpr (V == 1) return launch_fwd<D, V, 64, 1>(a);
     return ELX_E_SIZE;
 }
 
@@ -477,11 +488,11 @@ struct Bwd {
     hipStream_t stream;
 };
 
-// wavefronts per row of the backward pass: 8 elements per lane, 4 where they are loaded one by one
-template <int V>
+// Wavefronts per row of the backward pass: 8 elements per lane.  With 16 there is no room for the next rows (8192 x 4096 bf16:
+// 42 us against 38); with 4 of one element each, more wavefronts wait for each other (8191 x 2049 fp16: 58 against 49).
 uint32_t bwd_waves(uint32_t cols) {
     uint32_t w = 1;
-    while (w < 16 && w * kWave * (V == 1 ? 4 : 8) < cols) w *= 2;
+    while (w < 16 && w * kWave * 8 < cols) w *= 2;
     return w;
 }
 
@@ -514,23 +525,27 @@ int dispatch_bwd(const Bwd &a) {
     if (a.cols <= 8 * V) return launch_bwd<D, V, 1, 1, 8>(a);
     if (a.cols <= 16 * V) return launch_bwd<D, V, 1, 1, 16>(a);
     if (a.cols <= 32 * V) return launch_bwd<D, V, 1, 1, 32>(a);
-    const uint32_t waves = bwd_waves<V>(a.cols);
+    const uint32_t waves = bwd_waves(a.cols);
     const uint32_t n = (a.cols + waves * kWave * V - 1) / (waves * kWave * V);
 #define ELX_CASE(WAVES, ACCESSES)                                                  \
-    if constexpr (ACCESSES * V <= (WAVES == 16 ? 16 : V == 1 ? 4 : 8))             \
+    if constexpr (ACCESSES * V <= (WAVES == 16 ? 16 : 8))                           \
         if (waves == WAVES && n <= ACCESSES) return launch_bwd<D, V, ACCESSES, WAVES>(a);
     ELX_CASE(1, 1)
     ELX_CASE(1, 2)
     ELX_CASE(1, 4)
+    ELX_CASE(1, 8)
     ELX_CASE(2, 1)
     ELX_CASE(2, 2)
     ELX_CASE(2, 4)
+    ELX_CASE(2, 8)
     ELX_CASE(4, 1)
     ELX_CASE(4, 2)
     ELX_CASE(4, 4)
+    ELX_CASE(4, 8)
     ELX_CASE(8, 1)
     ELX_CASE(8, 2)
     ELX_CASE(8, 4)
+    ELX_CASE(8, 8)
     ELX_CASE(16, 1)
     ELX_CASE(16, 2)
     ELX_CASE(16, 4)

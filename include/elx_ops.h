@@ -115,7 +115,7 @@ int elx_layer_norm_bwd(const void *dy, const void *x, const void *w, const float
  * fp16, bf16); indices are 4- or 8-byte integers.
  *   forward   out[i] = scale * table[index[i]], multiplied in fp32 and rounded once.  An index outside [0, vocab) reads
  *             nothing; its row of `out` is NaN.
- *   backward  dtable[v] = scale * (sum of dy[i] over index[i] == v), summed in fp32 in the order of the tokens and rounded
+ *   backward  dtable[v] = scale * (sum of dy[i] over index[i] == v), summed in fp32 in a fixed order and rounded
  *             once; rows that no token names are zero.  All of dtable is written.  Tokens whose index is `padding` (< 0:
  *             none) or outside the table add nothing.  Rows of dy are `dy_stride` elements apart.  The workspace
  *             (elx_embedding_bwd_workspace() bytes, 16-byte aligned, contents ignored) holds the sorted tokens and partial sums.

@@ -273,3 +273,52 @@ def test_the_module_runs_the_kernel_and_falls_back(monkeypatch):
     sparse = ea.FusedEmbedding(30, 16, sparse=True).to(DEV)
     sparse(index).sum().backward()
     assert sparse.weight.grad.is_sparse and len(calls) == 2
+
+
+@pytest.mark.parametrize('tokens', [9000, 140000])
+def test_large_vocabularies_and_many_tokens(tokens):
+    """Three and four passes of the sort over several workgroups, up to the largest table; runs of one to many tokens."""
+    for vocab, dtype in (((1 << 20) + 77, torch.float32), (1 << 30, torch.bfloat16)):
+        g = torch.Generator(device=DEV).manual_seed(tokens)
+        index = torch.randint(0, vocab, (tokens, ), generator=g, device=DEV)
+        index[::3] = index[:5][torch.randint(0, 5, (len(index[::3]), ), generator=g, device=DEV)]
+        index[7], index[8], index[9] = vocab - 1, 0, vocab - 1
+        table = torch.zeros(vocab, 2, dtype=dtype, device=DEV)
+        dy = torch.randn(tokens, 2, generator=g, device=DEV).to(dtype)
+        d = run(index, table, dy)[1]
+        named, inverse, count = torch.unique(index, return_inverse=True, return_counts=True)
+        want = torch.zeros(len(named), 2, dtype=torch.float64, device=DEV).index_add_(0, inverse, dy.double())
+        size = torch.zeros(len(named), 2, dtype=torch.float64, device=DEV).index_add_(0, inverse, dy.double().abs())
+        tol = 2.0**-24 * (count[:, None] + 2) * size + half_step(dtype, want)
+        assert torch.all((d[named].double() - want).abs() <= tol)
+        d[named] = 0
+        assert not d.any()
+
+
+def test_hooks_that_hand_back_another_tensor_are_refused():
+    index, table, dy = make(70, 40, 16, torch.float32)
+    for unpack in (lambda t: t.int(), lambda t: t.cpu(), lambda t: t[:-1], lambda t: t.float()):
+        table.requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y = ea.embedding(index, table)
+        with pytest.raises(RuntimeError, match='came back'):
+            y.backward(dy)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: torch.stack([t, t], 1)[:, 0]):    # another layout is fine
+        y = ea.embedding(index, table)
+    assert torch.equal(torch.autograd.grad(y, table, dy)[0], run(index, table.detach(), dy)[1])
+
+
+def test_transforms_go_to_torch_or_are_refused():
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    index, table, _ = make(20, 30, 16, torch.float32)
+    emb = ea.FusedEmbedding.from_pretrained(table, freeze=True)
+    emb.scale = 2.0
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(table, torch.ones_like(table))
+        with pytest.raises(NotImplementedError):
+            ea.embedding(index, dual)
+        assert torch.equal(emb(index), table[index] * 2)
+    assert torch.equal(make_fx(lambda t: emb(t))(index)(index + 1), table[index + 1] * 2)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: ea.embedding(index, t).sum())(table)
