@@ -322,3 +322,21 @@ def test_transforms_go_to_torch_or_are_refused():
     assert torch.equal(make_fx(lambda t: emb(t))(index)(index + 1), table[index + 1] * 2)
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda t: ea.embedding(index, t).sum())(table)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('cols', [1, 5, 64, 96, 768, 770, 2048])
+@pytest.mark.parametrize('tokens', [1, 2, 63, 64, 65, 257, 512, 1000, 1024, 1025, 2048, 2049])
+def test_batches_around_the_changes_of_method(tokens, cols, dtype):
+    """One launch without a sort, a sort by one workgroup, a sort by several: unique tokens, one token, two, and a padded half."""
+    index, table, dy = make(tokens, 3000, cols, dtype, seed=tokens + cols, skew=1)
+    index[:] = torch.randperm(3000, device=DEV)[:tokens]
+    check(index, table, dy, scale=0.5)
+    index[tokens // 2:] = 2999
+    check(index, table, dy, padding_idx=2999)
+    check(index, table, dy)
+    index[:] = torch.arange(tokens, device=DEV) % 2
+    check(index, table, dy)
+    index[:] = -7    # outside: no gradient at all
+    table.requires_grad_(False)
+    assert not run(index, table, dy)[1].any()
