@@ -11,14 +11,16 @@
 // sums are in fp32 (per lane, then inside the wavefront, then over wavefronts through LDS), the one rounding to the
 // tensor's type is at the store.
 //
-// Backward: a workgroup of 16 wavefronts has 16 / W rows in flight and walks over rows with a stride; each lane sums dw and
+// Backward of few rows: one launch, some workgroups for dx, some for dw and db (layer_norm_few_kernel).  Of many: a workgroup of
+// 16 wavefronts has 16 / W rows in flight and walks over rows with a stride; each lane sums dw and
 // db of its own columns in registers over all its rows.  The row groups of a workgroup are added up in LDS, one partial row
 // per workgroup goes to a workspace, and a second launch adds the partial rows up in a fixed order: no atomics, the same
 // result every time.
 //
 // Both passes are bound by HBM where rows are many: 16384 x 4096 fp32 takes 93 us forward and 116 us backward from memory
 // (0.54 and 0.81 GB: 5.8 and 6.9 TB/s; 77 us forward where the cache holds a part), 8192 x 2048 bf16 12.3 and 19.6 us, where
-// the start and the end of a launch show.  A single row takes 2 us forward.  dw and db cost a second launch of 4 to 5 us.
+// the start and the end of a launch show.  A single row takes 2 us forward.  dw and db of many rows
+// cost a second launch of 4 to 5 us; 512 x 2048 bf16 takes 3.7 and 5.1 us.
 #include "elx_ops_device.h"
 
 using namespace elx_ops;
@@ -414,6 +416,118 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_fold_kernel(const floa
     }
 }
 
+// Few rows: dx and the sums over rows side by side in one launch; mean and rstd are there, so neither needs the other.  The
+// first `chunks` workgroups take `col_lanes` * V columns of dw and db each, over all rows; those behind them rows of dx.
+constexpr int kFewThreads = 4 * kWave;
+
+template <int D, int V, int N, int W, int L>
+__global__ __launch_bounds__(kFewThreads) void layer_norm_few_kernel(
+    const typename Elem<D>::scalar *__restrict__ dy, const typename Elem<D>::scalar *__restrict__ x,
+    const typename Elem<D>::scalar *__restrict__ w, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
+    typename Elem<D>::scalar *__restrict__ dx, typename Elem<D>::scalar *__restrict__ dw, typename Elem<D>::scalar *__restrict__ db,
+    uint32_t rows, uint32_t cols, uint64_t dy_stride, uint64_t x_stride, uint32_t chunks, uint32_t col_lanes) {
+    typedef typename Pack<D, V>::type pack_t;
+    static_assert(W <= 4, "a workgroup has four wavefronts");
+    if (blockIdx.x < chunks) {
+        constexpr uint32_t kAhead = 4;
+        __shared__ float sums[2][kFewThreads * V];
+        const uint32_t groups = kFewThreads / col_lanes, width = col_lanes * V;
+        const uint32_t group = threadIdx.x / col_lanes, c0 = blockIdx.x * width, c = c0 + threadIdx.x % col_lanes * V;
+        float sw[V], sb[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) sw[k] = sb[k] = 0.0f;
+        for (uint32_t r0 = group; r0 < rows; r0 += groups * kAhead) {
+            pack_t px[kAhead], pg[kAhead];
+            float mean[kAhead], rstd[kAhead];
+#pragma unroll
+            for (uint32_t j = 0; j < kAhead; ++j) {    // on their way at once
+                const uint32_t row = r0 + j * groups;
+                px[j] = pg[j] = pack_t{};
+                mean[j] = rstd[j] = 0.0f;
+                if (row < rows && c < cols) {
+                    px[j] = *reinterpret_cast<const pack_t *>(x + row * x_stride + c);
+                    pg[j] = *reinterpret_cast<const pack_t *>(dy + row * dy_stride + c);
+                    mean[j] = mean_in[row];
+                    rstd[j] = rstd_in[row];
+                }
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < kAhead; ++j) {
+                float h[V], g[V];
+                unpack<D, V>(px[j], h);
+                unpack<D, V>(pg[j], g);
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    sw[k] = fmaf(g[k], (h[k] - mean[j]) * rstd[j], sw[k]);
+                    sb[k] += g[k];
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            sums[0][threadIdx.x * V + k] = sw[k];
+            sums[1][threadIdx.x * V + k] = sb[k];
+        }
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < 2 * width; i += kFewThreads) {
+            const uint32_t which = i / width, at = i % width;
+            float s = 0.0f;
+#pragma unroll 16
+            for (uint32_t g = 0; g < groups; ++g) s += sums[which][g * width + at];
+            typename Elem<D>::scalar *out = which ? db : dw;
+            if (out && c0 + at < cols) out[c0 + at] = Elem<D>::from_f32(s);
+        }
+        return;
+    }
+    constexpr int kGroups = 4 / W * (kWave / L);    // rows of a workgroup
+    __shared__ float part[2][kGroups][W];
+    const int wave = threadIdx.x / kWave % W, lane = threadIdx.x % L;
+    const int group = threadIdx.x / kWave / W * (kWave / L) + threadIdx.x % kWave / L;
+    const uint32_t row = (blockIdx.x - chunks) * kGroups + group;
+    const bool live = row < rows;
+    const float mean = live ? mean_in[row] : 0.0f, rstd = live ? rstd_in[row] : 0.0f;
+    float h[N][V], t[N][V], st = 0.0f, sth = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const uint32_t c = ((uint32_t)(n * W + wave) * L + lane) * V;
+#pragma unroll
+        for (int k = 0; k < V; ++k) h[n][k] = t[n][k] = 0.0f;
+        if (live && c < cols) {
+            unpack<D, V>(*reinterpret_cast<const pack_t *>(x + row * x_stride + c), h[n]);
+            unpack<D, V>(*reinterpret_cast<const pack_t *>(dy + row * dy_stride + c), t[n]);
+            if (w) {
+                float wt[V];
+                unpack<D, V>(*reinterpret_cast<const pack_t *>(w + c), wt);
+#pragma unroll
+                for (int k = 0; k < V; ++k) t[n][k] *= wt[k];
+            }
+#pragma unroll
+            for (int k = 0; k < V; ++k) h[n][k] = (h[n][k] - mean) * rstd;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            st += t[n][k];
+            sth = fmaf(t[n][k], h[n][k], sth);
+        }
+    const float inv = 1.0f / (float)cols;
+    st = row_sum<W, L>(st, part[0][group], wave) * inv;
+    sth = row_sum<W, L>(sth, part[1][group], wave) * inv;
+    if (!live) return;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const uint32_t c = ((uint32_t)(n * W + wave) * L + lane) * V;
+        if (c < cols) {
+            float o[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) o[k] = (t[n][k] - st - h[n][k] * sth) * rstd;
+            __builtin_nontemporal_store(pack<D, V>(o), reinterpret_cast<pack_t *>(dx + (uint64_t)row * cols + c));
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------------------------
@@ -442,40 +556,50 @@ int launch_fwd(const Fwd &a) {
     return (int)hipGetLastError();
 }
 
+template <int N, int W, int L = kWave>
+struct shape {    // accesses per lane, wavefronts per row, lanes per row of a wavefront
+    static constexpr int accesses = N, waves = W, lanes = L;
+};
+
 // wavefronts per row and accesses per lane, the latter rounded up to what is compiled
-template <int D, int V>
-int dispatch_fwd(const Fwd &a) {
-    const uint32_t accesses = (a.cols + kWave * V - 1) / (kWave * V);    // wavefront-wide accesses of a row
+template <int V, typename F>
+int dispatch_rows(uint64_t rows, uint32_t cols, F &&launch) {
+    const uint32_t accesses = (cols + kWave * V - 1) / (kWave * V);    // wavefront-wide accesses of a row
     // Four wavefronts read a long row in a quarter of the steps, one wavefront needs no barrier:
     //   16384 x 4096 fp32   77 us with four, 93 with one      32768 x 2048 bf16   46 us with four, 42 with one
     //   32768 x 4096 bf16   79              100                8192 x 2048 bf16   14              10.6
     //    8191 x 1025 fp16   18               25                8191 x 1023 fp16   13.9            12.6
     // With few rows it is the steps that count (1024 x 2048 bf16: 4.5 us with four, 5.5 with one; 4096 x 2048: 7.1, 6.8).
-    if (accesses >= (V == 1 ? 17 : 8) || (a.rows < 4096 && accesses >= 4)) {
+    if (accesses >= (V == 1 ? 17 : 8) || (rows < 4096 && accesses >= 4)) {
         const uint32_t n = (accesses + 3) / 4;
-        if (n <= 1) return launch_fwd<D, V, 1, 4>(a);
-        if (n <= 2) return launch_fwd<D, V, 2, 4>(a);
-        if (n <= 4) return launch_fwd<D, V, 4, 4>(a);
-        if (n <= 8) return launch_fwd<D, V, 8, 4>(a);
+        if (n <= 1) return launch(shape<1, 4>());
+        if (n <= 2) return launch(shape<2, 4>());
+        if (n <= 4) return launch(shape<4, 4>());
+        if (n <= 8) return launch(shape<8, 4>());
         if constexpr (V <= 4)
-            if (n <= 16) return launch_fwd<D, V, 16, 4>(a);
+            if (n <= 16) return launch(shape<16, 4>());
         if constexpr (V == 1) {
-            if (n <= 32) return launch_fwd<D, V, 32, 4>(a);
-            if (n <= 64) return launch_fwd<D, V, 64, 4>(a);
+            if (n <= 32) return launch(shape<32, 4>());
+            if (n <= 64) return launch(shape<64, 4>());
         }
         return ELX_E_SIZE;
     }
-    if (a.cols <= 4 * V) return launch_fwd<D, V, 1, 1, 4>(a);
-    if (a.cols <= 8 * V) return launch_fwd<D, V, 1, 1, 8>(a);
-    if (a.cols <= 16 * V) return launch_fwd<D, V, 1, 1, 16>(a);
-    if (a.cols <= 32 * V) return launch_fwd<D, V, 1, 1, 32>(a);
-    if (accesses <= 1) return launch_fwd<D, V, 1, 1>(a);
-    if (accesses <= 2) return launch_fwd<D, V, 2, 1>(a);
-    if (accesses <= 4) return launch_fwd<D, V, 4, 1>(a);
-    if (accesses <= 8) return launch_fwd<D, V, 8, 1>(a);
+    if (cols <= 4 * V) return launch(shape<1, 1, 4>());
+    if (cols <= 8 * V) return launch(shape<1, 1, 8>());
+    if (cols <= 16 * V) return launch(shape<1, 1, 16>());
+    if (cols <= 32 * V) return launch(shape<1, 1, 32>());
+    if (accesses <= 1) return launch(shape<1, 1>());
+    if (accesses <= 2) return launch(shape<2, 1>());
+    if (accesses <= 4) return launch(shape<4, 1>());
+    if (accesses <= 8) return launch(shape<8, 1>());
     if constexpr (V == 1)
-        if (accesses <= 16) return launch_fwd<D, V, 16, 1>(a);
+        if (accesses <= 16) return launch(shape<16, 1>());
     return ELX_E_SIZE;
+}
+
+template <int D, int V>
+int dispatch_fwd(const Fwd &a) {
+    return dispatch_rows<V>(a.rows, a.cols, [&](auto s) { return launch_fwd<D, V, s.accesses, s.waves, s.lanes>(a); });
 }
 
 struct Bwd {
@@ -501,11 +625,7 @@ int launch_bwd(const Bwd &a) {
     typedef typename Elem<D>::scalar T;
     constexpr uint32_t groups = kBwdWaves / W * (kWave / L);
     const uint64_t want = (a.rows + groups - 1) / groups;
-    uint32_t blocks = (uint32_t)(want < kBwdBlocks ? want : kBwdBlocks);
-    // The partial rows of a workgroup are 16 bytes a column, written and read: where rows are few, fewer workgroups with
-    // more rows each, so that the partial rows stay below half of the tensors (300 x 11008 bf16: 31 us with 256 workgroups).
-    const uint64_t most = a.rows * sizeof(T) * 3 / 32;
-    if (a.partials && blocks > 64 && blocks > most) blocks = most < 64 ? 64 : (uint32_t)most;
+    const uint32_t blocks = (uint32_t)(want < kBwdBlocks ? want : kBwdBlocks);
     auto kernel = layer_norm_bwd_kernel<D, V, N, W, L, false>;
     if constexpr (V > 1) {
         if (2 * a.rows * a.cols * sizeof(T) > kCacheBytes) kernel = layer_norm_bwd_kernel<D, V, N, W, L, true>;
@@ -519,8 +639,30 @@ int launch_bwd(const Bwd &a) {
     return (int)hipGetLastError();
 }
 
+// Up to that many rows go in one launch (512 x 2048 bf16: 5.1 us against 9.8 in two, 1024 rows 6.9 against 10.9; 1400 rows of
+// 4096 17 against 15.7), with 64 or 128 bytes of a row per workgroup of the sums: the narrower, the more workgroups, the wider,
+// the better the reads (1024 x 2048 bf16 6.9 us with 64 and 9.4 with 128, 1024 x 11008 bf16 26 and 20).
+constexpr uint64_t kFewRows = 1024;
+constexpr uint32_t kNarrowBytes = 6144;    // of a row
+
+template <int D, int V, int N, int W, int L>
+int launch_few(const Bwd &a) {
+    typedef typename Elem<D>::scalar T;
+    constexpr uint32_t groups = 4 / W * (kWave / L);
+    const uint32_t col_lanes = a.cols * sizeof(T) <= kNarrowBytes ? 4 : 8;
+    const uint32_t width = col_lanes * V, rows = (uint32_t)a.rows;
+    const uint32_t chunks = a.dw || a.db ? (a.cols + width - 1) / width : 0;
+    hipLaunchKernelGGL((layer_norm_few_kernel<D, V, N, W, L>), dim3(chunks + (a.dx ? (rows + groups - 1) / groups : 0)), dim3(kFewThreads), 0,
+                       a.stream, (const T *)a.dy, (const T *)a.x, (const T *)a.w, a.mean, a.rstd, (T *)a.dx, (T *)a.dw, (T *)a.db, rows,
+                       a.cols, a.dy_stride, a.x_stride, chunks, col_lanes);
+    return (int)hipGetLastError();
+}
+
+
 template <int D, int V>
 int dispatch_bwd(const Bwd &a) {
+    if (a.rows <= kFewRows)
+        return dispatch_rows<V>(a.rows, a.cols, [&](auto s) { return launch_few<D, V, s.accesses, s.waves, s.lanes>(a); });
     if (a.cols <= 4 * V) return launch_bwd<D, V, 1, 1, 4>(a);
     if (a.cols <= 8 * V) return launch_bwd<D, V, 1, 1, 8>(a);
     if (a.cols <= 16 * V) return launch_bwd<D, V, 1, 1, 16>(a);

@@ -404,3 +404,21 @@ def test_transforms_go_to_torch_or_are_refused():
                  lambda: torch.func.grad(lambda t: ea.layer_norm(x, t, b).sum())(w)):
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows', [2, 15, 17, 255, 1023, 1024, 1025])
+@pytest.mark.parametrize('cols', [8, 64, 769, 2049, 3080, 11008])
+def test_rows_around_the_change_of_method(rows, cols, dtype):
+    """One launch for dx and the sums, or two; strided rows; each gradient alone."""
+    x, w, b, dy = inputs(rows, cols, dtype, seed=rows + cols)
+    wide = torch.zeros(rows, cols + 8, dtype=dtype, device=DEV)
+    wide[:, :cols] = x
+    x = wide[:, :cols].detach()
+    got = run(x, w, b, dy)
+    ref = reference(x, w, b, dy, 1e-5, dtype)
+    for name, t in zip(('y', 'dx', 'dw', 'db'), got):
+        check(t, *ref[name], name)
+    y = ea.layer_norm(x, w, b)
+    for i, leaf in enumerate((x, w, b)):
+        assert torch.equal(torch.autograd.grad(y, leaf, dy, retain_graph=True)[0], got[1 + i])
