@@ -2,7 +2,8 @@
 //
 //   y[i] = round(scale * W[index[i]])            dW[v] = round(scale * sum of dy[i] over index[i] = v)
 //
-// Forward is a gather: every row read and written once, 16 bytes per lane where the alignment allows.
+// Forward is a gather: every row read and written once, 16 bytes per lane where the alignment allows.  16384 tokens of 2048
+// bf16 columns take 19 us (127 MB: 6.6 TB/s), 8 tokens 2.5 us.
 //
 // Backward sums the rows of dy that belong to one row of the table in a fixed order, in fp32, and rounds once.  Few tokens take
 // one launch (direct_kernel).  For more, to have the rows of an index side by side, the tokens are sorted: a stable radix sort of
@@ -12,6 +13,8 @@
 //                row, a run that reaches over an end of the tile leaves an fp32 partial row; the workgroups behind these
 //                clear the rows that no token names, which the sorted tokens tell them: dW is written once;
 //   join_kernel  adds up the partial rows of the runs over several tiles (a frequent token), in a fixed order.
+// 16384 tokens of a 50272 x 2048 bf16 table take 3 + 2 x 7 us of sorting, 50 of sums and clearing (270 MB: 5.4 TB/s, of which 204
+// are written) and 6 of joining; 8191 tokens of 32000 x 4096 fp32 5 + 2 x 6, 118 (631 MB) and 6.
 // No atomics on values: the result is the same every time, and a token that fills the batch is summed by many workgroups.
 // (Clearing dW beside the sort instead, in the idle workgroups of its launches, made the sort three times slower -- its
 // chain of small reads waits behind the stores -- and wrote the touched rows twice: 89 us against 70 for 16384 tokens in a
