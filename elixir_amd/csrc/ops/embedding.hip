@@ -324,8 +324,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(Keys in, uint3
 
 // Tokens of a tile.  Few elements: short tiles, the launch lasts as long as its longest chain of them (768 columns of fp16:
 // 1021 tokens 25 us with 8, 33 with 24; 8192 tokens 38 and 46; 16384 tokens 42 and 45).  Many: long ones, every end of a tile
-// that cuts a run costs two fp32 rows (16384 x 2048 bf16: 74 us with 8, 69 with 24, 75 with 32, whose rows take too many
-// registers; 8192 x 4096 fp32: 147 with 8, 136 with 24).
+// that cuts a run costs two fp32 rows (16384 x 2048 bf16: 69 us with 8, 65 with 24, 70 with 32, whose rows take too many
+// registers; 8192 x 4096 fp32: 134 with 8, 119 with 24, 130 with 16).
 constexpr uint32_t kTileFew = 8, kTileMany = 24;
 constexpr uint64_t kFewElems = 1ull << 24;
 constexpr int kSumThreads = 256;    // at most
@@ -370,9 +370,15 @@ __device__ __forceinline__ bool names(const uint32_t *__restrict__ keys, uint32_
     return lo < end && keys[lo] == key;
 }
 
-// Clears those of the rows [row, row + count) that `named` does not name, in units of `unit` bytes.
+// dy that fits the memory-side cache is likely to be there, left by the launches before: ordinary loads (8192 x 4096 fp32: 119 us
+// against 131 with non-temporal ones, 65536 x 768 bf16 64 against 77); what does not streams past it (1048576 x 128 bf16: 270 us
+// against 277).  Where dW fits beside it rows are cleared there, too (8192 tokens of 50272 x 2048 bf16, 239 MB: 54 us against 63;
+// 16384 tokens, 273 MB: 65 and 65; of 32000 x 4096 bf16 104 against 86).
+constexpr uint64_t kCacheBytes = 256ull << 20;
+
+// Clears those of the rows [row, row + count) that `named` does not name, in units of `unit` bytes; `keep`: in the cache.
 __device__ __forceinline__ void zero_rows(const uint32_t *named, uint32_t row, uint32_t count, char *base, uint32_t row_bytes,
-                                          uint32_t unit) {
+                                          uint32_t unit, bool keep) {
     const uint32_t threads = blockDim.x;
     const uint32_t units = row_bytes / unit;
     uint32_t r = threadIdx.x / units, u = threadIdx.x % units;
@@ -380,7 +386,9 @@ __device__ __forceinline__ void zero_rows(const uint32_t *named, uint32_t row, u
     while (r < count) {
         if (!(named[r / 32] >> (r % 32) & 1)) {
             char *to = base + (uint64_t)(row + r) * row_bytes + (uint64_t)u * unit;
-            if (unit == 16)
+            if (unit == 16 && keep)
+                *reinterpret_cast<u32x4 *>(to) = u32x4{0, 0, 0, 0};
+            else if (unit == 16)
                 __builtin_nontemporal_store(u32x4{0, 0, 0, 0}, reinterpret_cast<u32x4 *>(to));
             else if (unit == 4)
                 *reinterpret_cast<uint32_t *>(to) = 0;
@@ -398,7 +406,7 @@ __device__ __forceinline__ void zero_rows(const uint32_t *named, uint32_t row, u
 
 // Clears those of the rows [row, row + count) that no token names.
 __device__ __forceinline__ void clear_rows(const uint32_t *__restrict__ keys, uint32_t n, uint32_t row, uint32_t count, char *base,
-                                           uint32_t row_bytes, uint32_t unit) {
+                                           uint32_t row_bytes, uint32_t unit, bool keep) {
     __shared__ uint32_t named[kFillRows / 32];
     __shared__ uint32_t bounds[2];
     const uint32_t threads = blockDim.x, wave = threadIdx.x / kWave, waves = threads / kWave;
@@ -424,7 +432,7 @@ __device__ __forceinline__ void clear_rows(const uint32_t *__restrict__ keys, ui
             if (names(keys, lo, hi, row + r)) atomicOr(&named[r / 32], 1u << (r % 32));
     }
     __syncthreads();
-    zero_rows(named, row, count, base, row_bytes, unit);
+    zero_rows(named, row, count, base, row_bytes, unit, keep);
 }
 
 template <typename F, uint32_t... I>
@@ -438,10 +446,10 @@ __device__ __forceinline__ void each(F &&f) {
 }
 
 struct Clear {    // the workgroups behind those of the tiles
-    uint32_t tile_blocks, chunks, rows_per_block, row_bytes, unit;
+    uint32_t tile_blocks, chunks, rows_per_block, row_bytes, unit, keep;
 };
 
-template <int D, int V, uint32_t kTokens>
+template <int D, int V, uint32_t kTokens, bool STREAM>
 __global__ __launch_bounds__(kSumThreads) void sum_kernel(const uint32_t *__restrict__ keys, const uint32_t *__restrict__ positions,
                                                           uint32_t n, uint32_t vocab, const typename Elem<D>::scalar *__restrict__ dy,
                                                           uint64_t dy_stride, uint32_t cols, float scale,
@@ -451,7 +459,7 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const uint32_t *__rest
     if (blockIdx.x >= clear.tile_blocks) {
         const uint32_t row = (blockIdx.x - clear.tile_blocks) * clear.rows_per_block;
         const uint32_t count = vocab - row < clear.rows_per_block ? vocab - row : clear.rows_per_block;
-        clear_rows(keys, n, row, count, reinterpret_cast<char *>(dtable), clear.row_bytes, clear.unit);
+        clear_rows(keys, n, row, count, reinterpret_cast<char *>(dtable), clear.row_bytes, clear.unit, clear.keep);
         return;
     }
     const uint32_t tile = blockIdx.x / clear.chunks;
@@ -477,9 +485,10 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(const uint32_t *__rest
     // behind a store would wait for memory to take the store in.
     typename row_t::type rows[kTokens];
     each<kTokens>([&](auto j) {
-        if (j < count && mine)
-            rows[j] = __builtin_nontemporal_load(
-                reinterpret_cast<const typename row_t::type *>(dy + (uint64_t)position_of(j) * dy_stride + c));
+        if (j < count && mine) {
+            const auto *from = reinterpret_cast<const typename row_t::type *>(dy + (uint64_t)position_of(j) * dy_stride + c);
+            rows[j] = STREAM ? __builtin_nontemporal_load(from) : *from;
+        }
     });
     each<kTokens>([&](auto j) {
         if (j >= count) return;
@@ -542,7 +551,7 @@ __global__ __launch_bounds__(kDirectThreads) void direct_kernel(Keys in, uint32_
             if (key < count) atomicOr(&named[key / 32], 1u << (key % 32));
         }
         __syncthreads();
-        zero_rows(named, row, count, reinterpret_cast<char *>(dtable), clear.row_bytes, clear.unit);
+        zero_rows(named, row, count, reinterpret_cast<char *>(dtable), clear.row_bytes, clear.unit, clear.keep);
         return;
     }
     __shared__ uint64_t same[kDirectTokens / kWave];    // the tokens of this index
@@ -589,8 +598,7 @@ __global__ __launch_bounds__(kDirectThreads) void direct_kernel(Keys in, uint32_
 #pragma unroll
             for (uint32_t j = 0; j < kAhead; ++j)
                 if (k + j * groups < count)
-                    rows[j] = __builtin_nontemporal_load(
-                        reinterpret_cast<const pack_t *>(dy + (uint64_t)token_of[k + j * groups] * dy_stride + c));
+                    rows[j] = *reinterpret_cast<const pack_t *>(dy + (uint64_t)token_of[k + j * groups] * dy_stride + c);
 #pragma unroll
             for (uint32_t j = 0; j < kAhead; ++j)
                 if (k + j * groups < count) {
@@ -762,10 +770,11 @@ uint64_t round256(uint64_t x) { return (x + 255) & ~255ull; }
 
 // the clearing workgroups of `threads` threads behind `tile_blocks` others; returns how many
 template <int D>
-uint64_t plan_clear(Clear *clear, uint64_t vocab, uint32_t cols, const void *dtable, uint32_t threads) {
+uint64_t plan_clear(Clear *clear, uint64_t n, uint64_t vocab, uint32_t cols, const void *dtable, uint32_t threads) {
     const uint32_t es = elem_size(D);
     clear->row_bytes = cols * es;
     clear->unit = clear->row_bytes % 16 == 0 && aligned16(dtable) ? 16 : es;
+    clear->keep = (n + vocab) * clear->row_bytes <= kCacheBytes;
     const uint32_t rows = kFillBytes * threads / clear->row_bytes;
     clear->rows_per_block = rows < 1 ? 1 : rows > kFillRows ? kFillRows : rows;
     return (vocab + clear->rows_per_block - 1) / clear->rows_per_block;
@@ -791,7 +800,7 @@ int launch_direct(const Keys &in, const Grad &a) {
     Clear clear;
     clear.chunks = direct_chunks<V>(a.cols);
     clear.tile_blocks = (uint32_t)a.n * clear.chunks;
-    const uint64_t clear_blocks = plan_clear<D>(&clear, a.vocab, a.cols, a.dtable, kDirectThreads);
+    const uint64_t clear_blocks = plan_clear<D>(&clear, a.n, a.vocab, a.cols, a.dtable, kDirectThreads);
     hipLaunchKernelGGL((direct_kernel<D, V>), dim3((uint32_t)(clear.tile_blocks + clear_blocks)), dim3(kDirectThreads), 0, a.stream, in,
                        (uint32_t)a.n, (const T *)a.dy, a.dy_stride, a.cols, a.scale, (T *)a.dtable,
                        lanes_for((a.cols + V - 1) / V, kDirectLanes), clear);
@@ -807,15 +816,14 @@ int launch_sums(const Shape &s, const uint32_t *keys, const uint32_t *positions,
     clear.tile_blocks = s.tiles * clear.chunks;
     // whole wavefronts, no more than the columns need: idle ones would take the place of other tiles
     const dim3 threads(((accesses + clear.chunks - 1) / clear.chunks + kWave - 1) / kWave * kWave);
-    const uint64_t clear_blocks = plan_clear<D>(&clear, a.vocab, a.cols, a.dtable, threads.x);
+    const uint64_t clear_blocks = plan_clear<D>(&clear, a.n, a.vocab, a.cols, a.dtable, threads.x);
     const dim3 grid((uint32_t)(clear.tile_blocks + clear_blocks));
     const uint32_t n = (uint32_t)a.n, vocab = (uint32_t)a.vocab;
-    if (s.tokens == kTileFew)
-        hipLaunchKernelGGL((sum_kernel<D, V, kTileFew>), grid, threads, 0, a.stream, keys, positions, n, vocab, (const T *)a.dy, a.dy_stride,
-                           a.cols, a.scale, (T *)a.dtable, partials, clear);
-    else
-        hipLaunchKernelGGL((sum_kernel<D, V, kTileMany>), grid, threads, 0, a.stream, keys, positions, n, vocab, (const T *)a.dy, a.dy_stride,
-                           a.cols, a.scale, (T *)a.dtable, partials, clear);
+    auto kernel = sum_kernel<D, V, kTileFew, false>;    // kFewElems elements fit the cache
+    if (s.tokens == kTileMany)
+        kernel = a.n * a.cols * sizeof(T) > kCacheBytes ? sum_kernel<D, V, kTileMany, true> : sum_kernel<D, V, kTileMany, false>;
+    hipLaunchKernelGGL(kernel, grid, threads, 0, a.stream, keys, positions, n, vocab, (const T *)a.dy, a.dy_stride, a.cols, a.scale,
+                       (T *)a.dtable, partials, clear);
     if (int rc = (int)hipGetLastError()) return rc;
     if (s.tiles < 2) return 0;
     constexpr int J = V > 1 ? 4 : 1;
