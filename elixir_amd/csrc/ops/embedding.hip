@@ -13,8 +13,8 @@
 //                row, a run that reaches over an end of the tile leaves an fp32 partial row; the workgroups behind these
 //                clear the rows that no token names, which the sorted tokens tell them: dW is written once;
 //   join_kernel  adds up the partial rows of the runs over several tiles (a frequent token), in a fixed order.
-// 16384 tokens of a 50272 x 2048 bf16 table take 3 + 2 x 7 us of sorting, 50 of sums and clearing (270 MB: 5.4 TB/s, of which 204
-// are written) and 6 of joining; 8191 tokens of 32000 x 4096 fp32 5 + 2 x 6, 118 (631 MB) and 6.
+// 16384 tokens of a 50272 x 2048 bf16 table take 4 + 2 x 6 us of sorting, 43 of sums and clearing (277 MB, of which 208 are
+// written: 6.4 TB/s) and 7 of joining; 8191 tokens of 32000 x 4096 fp32 5 + 2 x 6, 98 (646 MB) and 6.
 // No atomics on values: the result is the same every time, and a token that fills the batch is summed by many workgroups.
 // (Clearing dW beside the sort instead, in the idle workgroups of its launches, made the sort three times slower -- its
 // chain of small reads waits behind the stores -- and wrote the touched rows twice: 89 us against 70 for 16384 tokens in a
@@ -370,10 +370,12 @@ __device__ __forceinline__ bool names(const uint32_t *__restrict__ keys, uint32_
     return lo < end && keys[lo] == key;
 }
 
-// dy that fits the memory-side cache is likely to be there, left by the launches before: ordinary loads (8192 x 4096 fp32: 119 us
-// against 131 with non-temporal ones, 65536 x 768 bf16 64 against 77); what does not streams past it (1048576 x 128 bf16: 270 us
-// against 277).  Where dW fits beside it rows are cleared there, too (8192 tokens of 50272 x 2048 bf16, 239 MB: 54 us against 63;
-// 16384 tokens, 273 MB: 65 and 65; of 32000 x 4096 bf16 104 against 86).
+// dy that fits the memory-side cache is likely to be there, left by the launch before: ordinary loads (behind a launch that wrote
+// dy, 8191 x 4096 fp32: 119 us against 136 with non-temporal ones, 16384 x 2048 bf16 64 against 73, 65536 x 768 bf16 64 against
+// 77); what does not streams past it (1048576 x 128 bf16: 270 us against 277).  Where dW fits beside it rows are cleared there,
+// too, for its reader, the landing of the gradient: with a launch that reads dW right behind, 1021 tokens of 50257 x 768 fp16
+// take 45 us against 54, 16384 of 32000 x 1024 bf16 64 against 68 (alone 20 against 19 and 46 against 43); where it does not
+// fit it costs (16384 of 32000 x 4096 bf16 104 against 86).
 constexpr uint64_t kCacheBytes = 256ull << 20;
 
 // Clears those of the rows [row, row + count) that `named` does not name, in units of `unit` bytes; `keep`: in the cache.
