@@ -340,3 +340,49 @@ def test_batches_around_the_changes_of_method(tokens, cols, dtype):
     index[:] = -7    # outside: no gradient at all
     table.requires_grad_(False)
     assert not run(index, table, dy)[1].any()
+
+
+@pytest.mark.parametrize('tokens, cols', [(7, 64), (1000, 64), (1000, 5), (1500, 64), (5000, 64)])
+def test_graphs_of_every_method(tokens, cols):
+    """Two graphs in flight on two streams, each replayed on new inputs, against eager passes."""
+    graphs = []
+    for seed in range(2):
+        index, table, dy = make(tokens, 700, cols, torch.float16, seed=seed)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(index, table, dy, padding_idx=3)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(index, table, dy, padding_idx=3)
+        graphs.append((graph, out, (index, table, dy)))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for turn in range(1, 4):
+        new = [make(tokens, 700, cols, torch.float16, seed=10 * turn + i, skew=turn) for i in range(2)]
+        for (_, _, static), fresh in zip(graphs, new):
+            with torch.no_grad():
+                for s, t in zip(static, fresh):
+                    s.copy_(t)
+        torch.cuda.synchronize()
+        for (graph, _, _), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, out, _), fresh in zip(graphs, new):
+            assert all(torch.equal(a, e) for a, e in zip(out, run(*fresh, padding_idx=3))), turn
+
+
+def test_few_tokens_of_wide_and_long_tables():
+    """One launch where offsets pass 32 bits, and at the largest table."""
+    for vocab, cols, dtype in ((2**20 + 7, 4096, torch.bfloat16), (1 << 30, 4, torch.float16)):
+        index = torch.tensor([vocab - 1, 0, 5, vocab - 1, vocab // 2, 5, vocab], device=DEV)
+        dy = torch.randn(7, cols, device=DEV, dtype=torch.float32).to(dtype)
+        table = torch.zeros(vocab, cols, dtype=dtype, device=DEV)
+        d = run(index, table, dy)[1]
+        want = {vocab - 1: dy[0].double() + dy[3].double(), 0: dy[1].double(), 5: dy[2].double() + dy[5].double(), vocab // 2: dy[4].double()}
+        for row, value in want.items():
+            assert torch.all((d[row].double() - value).abs() <= 4 * 2.0**-24 * dy.abs().max().item() * 2 + half_step(dtype, value))
+            d[row] = 0
+        assert not d.any()
+        del d, table

@@ -422,3 +422,34 @@ def test_rows_around_the_change_of_method(rows, cols, dtype):
     y = ea.layer_norm(x, w, b)
     for i, leaf in enumerate((x, w, b)):
         assert torch.equal(torch.autograd.grad(y, leaf, dy, retain_graph=True)[0], got[1 + i])
+
+
+@pytest.mark.parametrize('rows, cols', [(1, 2048), (1024, 96), (1025, 96), (3000, 2048)])
+def test_graphs_of_both_methods(rows, cols):
+    """Two graphs in flight on two streams, each replayed on new inputs, against eager passes."""
+    graphs = []
+    for seed in range(2):
+        static = [t.detach() for t in inputs(rows, cols, torch.float16, seed=seed)]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(*static)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(*static)
+        graphs.append((graph, out, static))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for turn in range(1, 4):
+        new = [[t.detach() for t in inputs(rows, cols, torch.float16, seed=10 * turn + i)] for i in range(2)]
+        for (_, _, static), fresh in zip(graphs, new):
+            with torch.no_grad():
+                for s, t in zip(static, fresh):
+                    s.copy_(t)
+        torch.cuda.synchronize()
+        for (graph, _, _), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, out, _), fresh in zip(graphs, new):
+            assert all(torch.equal(a, e) for a, e in zip(out, run(*fresh))), turn
