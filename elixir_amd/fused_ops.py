@@ -6,8 +6,8 @@ The reference swaps ``F.layer_norm`` for a third party's fused kernel (elixir/ke
 embedding to torch.  Both functions take device tensors in fp32, fp16 or bf16, compute in fp32 and round once, run on the
 current stream of the tensors' device, allocate what they return (and, in backward, a workspace) through torch's allocator,
 synchronise nothing, and can be captured into a graph.  A gradient that is itself to be differentiated
-(``create_graph=True``) is computed by torch's own operators; forward-mode derivatives and tracing are refused.  What the functions cannot take they refuse; the modules fall
-back to torch instead, so that a model keeps running wherever it ran."""
+(``create_graph=True``) is computed by torch's own operators; forward-mode derivatives and tracing are refused.  What the
+functions cannot take they refuse; the modules fall back to torch instead, so that a model keeps running wherever it ran."""
 from typing import Optional, Sequence, Union
 
 import torch
@@ -44,7 +44,8 @@ def embedding(input: torch.Tensor, weight: torch.Tensor, padding_idx: Optional[i
     """Rows of ``weight`` named by ``input``, times ``scale`` (multiplied in fp32, rounded once).
 
     input: int64 or int32 device tensor of any shape, up to 2^26 tokens.  weight: [rows, cols] on the same device in fp32,
-        fp16 or bf16; it and the embedded tokens have up to 2^34 elements.  padding_idx: a row whose tokens add nothing to the gradient (negative: counted from the end).
+        fp16 or bf16; it and the embedded tokens have up to 2^34 elements.  padding_idx: a row whose tokens add nothing to
+        the gradient (negative: counted from the end).
     The gradient of ``weight`` is dense, summed in fp32 in a fixed order (the same bits every time) and rounded
     once.  The indices are not checked on the host: one outside the table gives a row of NaN and no gradient."""
     return (_ext or _load()).embedding(input, weight, padding_idx, scale)
