@@ -141,12 +141,15 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const bool want_b = (affine & 2) && ctx->needs_input_grad(edge++);
         Tensor dx, dw, db;
         if (at::GradMode::is_enabled()) {    // the gradient is to be differentiated: torch's operators
+            // With respect to aliases: the saved tensors carry their history, and where one of them is an ancestor of the
+            // other (one norm in two layers) the derivative would run on through it, a path that is the outer pass's.
+            const Tensor a = x.view_as(x), w = weight.defined() ? weight.view_as(weight) : weight;
             const Tensor b = want_b ? at::zeros(shape, x.options()).requires_grad_() : Tensor();
             variable_list leaves;
-            if (want_x) leaves.push_back(x);
-            if (want_w) leaves.push_back(weight);
+            if (want_x) leaves.push_back(a);
+            if (want_w) leaves.push_back(w);
             if (want_b) leaves.push_back(b);
-            const Tensor y = at::layer_norm(x, shape, weight, b, ctx->saved_data["eps"].toDouble());
+            const Tensor y = at::layer_norm(a, shape, w, b, ctx->saved_data["eps"].toDouble());
             auto got = torch::autograd::grad({y}, leaves, {grad}, std::nullopt, true);
             size_t i = 0;
             if (want_x) dx = got[i++];
