@@ -224,7 +224,8 @@ __device__ __forceinline__ void encode(const float (&m)[kVec], const float (&v)[
     uint32_t code[kVec];
 #pragma unroll
     for (int k = 0; k < kVec; ++k) {
-        const uint32_t t = __builtin_bit_cast(uint32_t, __builtin_ldexpf(v[k], 31 - ve));
+        // without its sign, which the code has no place for: a bit of it would land in the next element's code
+        const uint32_t t = __builtin_bit_cast(uint32_t, __builtin_ldexpf(__builtin_fabsf(v[k]), 31 - ve));
         code[k] = max((t + r[k]) >> 20, min(bv[k], 1u));
     }
     if (!whole) {

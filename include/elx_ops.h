@@ -45,7 +45,8 @@ const char *elx_ops_source_sha(void);
  *   key  = mix(block ^ mix(salt * 0x9E3779B9 + step))
  *   word = mix(key + lane * 0x9E3779B9)         lane = (element of the block) / 4
  *   r    = rotate_right(word, 8 * (element of the block mod 4)) >> 12
- * A value that is not zero never becomes zero: the next step would divide by eps alone.
+ * A value that is not zero never becomes zero: the next step would divide by eps alone.  exp_avg_sq is a sum of squares and
+ * its code has no sign: -0.0 is zero, and of a negative value, which only a checkpoint could bring, the magnitude is held.
  * A value that is not finite becomes NaN; its neighbours in the block keep theirs.
  */
 typedef struct ElxState8 {
