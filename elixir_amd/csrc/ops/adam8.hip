@@ -127,6 +127,9 @@ __device__ __forceinline__ void with_variant(const Hyper &h, const Unscale &us, 
 // ---------------------------------------------------------------------------------------------
 
 constexpr uint32_t kInf = 0x7F800000u;
+// The largest magnitude that does not take exponent 255, 1.75 * 2^127.  Under 255 the code above these stands for 2^128, which
+// fp32 does not hold: a finite value is held at 1.875 * 2^127 at most.
+constexpr uint32_t kOrdinary = 0x7F600000u, kAvgTop = 0x77u, kSqTop = 0xF7u;
 constexpr uint32_t kHalf = 1u << 19;    // r of rounding to nearest
 
 __device__ __forceinline__ uint32_t mix(uint32_t x) {
@@ -204,8 +207,8 @@ __device__ __forceinline__ void encode(const float (&m)[kVec], const float (&v)[
     }
     uint32_t mt = max(max(bm[0], bm[1]), max(bm[2], bm[3])), vt = max(max(bv[0], bv[1]), max(bv[2], bv[3]));
     wave_max(mt, vt);
-    const bool whole = max(mt, vt) < kInf;
-    if (!whole) {    // the exponents are those of the finite elements
+    const bool ordinary = max(mt, vt) <= kOrdinary;
+    if (!ordinary) {    // the exponents are those of the finite elements
         mt = vt = 0;
 #pragma unroll
         for (int k = 0; k < kVec; ++k) {
@@ -228,10 +231,14 @@ __device__ __forceinline__ void encode(const float (&m)[kVec], const float (&v)[
         const uint32_t t = __builtin_bit_cast(uint32_t, __builtin_ldexpf(__builtin_fabsf(v[k]), 31 - ve));
         code[k] = max((t + r[k]) >> 20, min(bv[k], 1u));
     }
-    if (!whole) {
+    if (!ordinary) {
 #pragma unroll
         for (int k = 0; k < kVec; ++k) {
-            if (bm[k] >= kInf) m_word = (m_word & ~(0xFFu << (8 * k))) | (0x7Fu << (8 * k));
+            uint32_t c = (m_word >> (8 * k)) & 0xFFu;
+            if (me == 255 && (c & 0x7Fu) > kAvgTop) c = (c & 0x80u) | kAvgTop;
+            if (bm[k] >= kInf) c = 0x7Fu;
+            m_word = (m_word & ~(0xFFu << (8 * k))) | (c << (8 * k));
+            if (ve == 255) code[k] = min(code[k], kSqTop);
             if (bv[k] >= kInf) code[k] = 0xFFu;
         }
     }

@@ -36,7 +36,8 @@ const char *elx_ops_source_sha(void);
  * E is the smallest exponent for which the largest finite magnitude of the block is at most 1.75 * 2^(E - 127), and for
  * E = 0, where fp32 has no implicit bit, at most 1.5 * 2^-127: (bits of the largest + 0x1FFFFF) >> 23.  The
  * scales are powers of two, so what the codes hold is exact in fp32 (and in bfloat16), and writing back what was read
- * changes no value.
+ * changes no value.  (Under E = 255 a code could stand for 2^128, which fp32 does not hold: what is finite is written as
+ * 1.875 * 2^127 at most.)
  * exp_avg_sq moves by (1 - beta2) of itself in a step, far less than the distance of two codes: rounded to nearest it
  * would never move.  It is rounded up or down at random with the right expectation: 20 bits r per element are added below
  * the mantissa that is kept and the sum is cut off.  The bits depend on (salt, element, step) alone, so a step gives the

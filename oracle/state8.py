@@ -52,6 +52,8 @@ def encode_avg(x: np.ndarray):
     e = exponent(x)
     scaled = np.ldexp(x, (135 - e)[:, None].astype(np.int32)).astype(np.float32)
     codes = torch.from_numpy(scaled).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+    over = (e == 255)[:, None] & ((codes & 0x7F) > 0x77)    # 2^128: the largest value of fp32 is below
+    codes = np.where(over, (codes & 0x80) | 0x77, codes)
     return np.where(np.isfinite(x), codes, 0x7F).astype(np.uint8), e
 
 
@@ -60,6 +62,7 @@ def encode_sq(x: np.ndarray, r: np.ndarray):
     e = exponent(x)
     bits = np.ldexp(x, (31 - e)[:, None].astype(np.int32)).astype(np.float32).view(np.uint32).astype(np.int64)
     codes = np.maximum((bits + r) >> 20, (x != 0).astype(np.int64))
+    codes = np.where((e == 255)[:, None], np.minimum(codes & 0xFF, 0xF7), codes)
     return np.where(np.isfinite(x), codes, 0xFF).astype(np.uint8), e
 
 

@@ -67,3 +67,46 @@ def test_a_checkpoint_with_such_values_spoils_no_neighbour():
             got.append(opt.read_moments(p[0] if isinstance(p, tuple) else p))
         assert all(torch.equal(a, b) for a, b in zip(*got))
         assert not got[1][1][places].any()
+
+
+LARGEST = float(np.finfo(np.float32).max)
+
+
+@pytest.mark.parametrize('top', [LARGEST, 1.9375 * 2.0**127, 1.875 * 2.0**127, 1.75 * 2.0**127])
+@pytest.mark.parametrize('moment', [0, 1])
+def test_what_is_finite_stays_finite(top, moment):
+    """Values next to the end of fp32, whose nearest code would stand for 2^128, between ordinary ones, an infinity and a NaN."""
+    x = np.random.default_rng(1).random((3, 256)).astype(np.float32) * np.float32(1e38)
+    x[0, [0, 77, 255]] = top
+    x[1, 3], x[1, 4], x[1, 5] = top, np.inf, np.nan
+    if moment == 0:
+        x[:, 1::2] *= -1
+    want, e = (S8.encode_sq(x, S8.HALF) if moment else S8.encode_avg(x))
+    codes, scales = write(x, moment)
+    got = to_np(codes).reshape(x.shape)
+    got = got if moment else np.where((got & 0x7F) == 0x7F, 0x7F, got)
+    assert np.array_equal(got, want) and np.array_equal(to_np(scales)[:, moment].astype(np.int64), e)
+    values = _read_state8(codes, codes, scales, 0, x.size, torch.float32, torch.device('cuda', 0))[moment]
+    finite = np.isfinite(x.reshape(-1))
+    back = to_np(values)
+    assert np.array_equal(np.isfinite(back), finite)
+    # half a step of three mantissa bits; held at 1.875 * 2^127 the largest number of fp32 is off by a whole one
+    assert np.all(np.abs(back[finite].astype(np.float64) / x.reshape(-1)[finite].astype(np.float64) - 1) <= 2.0**-4)
+    again, scales2 = write(back, moment)
+    assert torch.equal(again, codes) and torch.equal(scales2, scales)    # what was read is written back unchanged
+
+
+def test_steps_with_squares_next_to_the_end_of_fp32():
+    """exp_avg_sq of (1 - beta2) g^2 between 1.875 * 2^127 and the largest number: finite after every step, as in 32 bits."""
+    n = 512
+    p = torch.nn.Parameter(torch.zeros(n, device=DEV))
+    opt = ea.HybridAdam([p], lr=1e-3, betas=(0.9, 0.999), state_bits=8)
+    g = torch.full((n, ), 1e-3)
+    g[::7] = 5.75e20    # 0.001 g^2 = 3.306e38
+    g[3::7] = -5.7e20
+    for step in range(1, 4):
+        p.grad = (g if step == 1 else torch.full((n, ), 1e-3)).to(DEV)
+        opt.step()
+        m, v = opt.read_moments(p)
+        assert torch.isfinite(m).all() and torch.isfinite(v).all() and torch.isfinite(p).all(), step
+        assert v[::7].min() > 2.9e38 * 0.875
