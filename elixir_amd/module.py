@@ -111,9 +111,13 @@ def get_param_optim_data(param_data: torch.Tensor, param_dtype: torch.dtype, dev
     return param_data, optim_data
 
 
-def reserve_device_pool(nbytes: int, device: torch.device, minimum: int = 1 << 30) -> bool:
+POOL_MINIMUM = 1 << 30    # bytes of shards, master weights and 32-bit moments from which a set is worth a pool
+POOL_SLACK = 256 << 20    # rounding of the individual allocations, tables, workspaces
+
+
+def reserve_device_pool(nbytes: int, device: torch.device, minimum: int = POOL_MINIMUM, slack: int = POOL_SLACK) -> bool:
     """Takes ``nbytes`` of device memory from the driver in ONE allocation and hands it straight to
-    torch's caching allocator, which then carves the chunk shards, master weights and moments out of
+    torch's caching allocator, which then carves the chunk shards and master weights (or the moments) out of
     it.  Dozens of allocations of a gigabyte each, made in turn on a device whose memory other
     processes have used and released before, get less contiguous memory than one allocation for all
     of them, and the streaming kernels feel it: the same update launch over the LLaMA-7B set takes
@@ -121,7 +125,7 @@ def reserve_device_pool(nbytes: int, device: torch.device, minimum: int = 1 << 3
     for small sets and when that much memory is not free.  Returns whether it reserved."""
     if nbytes < minimum or device.type != 'cuda':
         return False
-    nbytes += 256 << 20    # rounding of the individual allocations, tables, workspaces
+    nbytes += slack
     free, _ = torch.cuda.mem_get_info(device)
     cached_free = torch.cuda.memory_reserved(device) - torch.cuda.memory_allocated(device)
     if nbytes > free + cached_free - (2 << 30):
@@ -186,6 +190,7 @@ class ElixirModule(nn.Module):
         self.reduce_always_fp32 = reduce_always_fp32
         self.output_fp32 = output_fp32
         self.reserve_memory = reserve_memory
+        self.pooled_elems = 0    # elements on the device of a set that is worth a pool: the optimizer reserves their moments
         self.buffer = None
 
         self.no_grad_state_dict = dict()
@@ -233,7 +238,10 @@ class ElixirModule(nn.Module):
             gpu_elems = sum(plan.chunk_size for plan in sr.param_chunk_plans
                             if torch.device(plan.kwargs.get('shard_device', device)).type == 'cuda')
             esize = torch.empty(0, dtype=self.dtype).element_size()
-            reserve_device_pool(gpu_elems * (esize + 4 + 8), device)    # shards, master, exp_avg, exp_avg_sq
+            if gpu_elems * (esize + 4 + 8) >= POOL_MINIMUM:
+                # shards and master weights; the moments are the optimizer's, which knows their width
+                reserve_device_pool(gpu_elems * (esize + 4), device, minimum=0)
+                self.pooled_elems = gpu_elems
 
         for plan in sr.param_chunk_plans:
             assert plan.chunk_dtype == self.dtype
