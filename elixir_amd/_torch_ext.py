@@ -12,10 +12,16 @@ LIB_PATH = os.path.join(_HERE, '_elx_torch.so')
 SOURCE = os.path.join(_HERE, 'csrc', 'torch', 'elx_torch.cpp')
 
 
+def source_files():
+    """What the extension is made from, in the order of the digest: its source and the headers it calls through."""
+    include = os.path.join(os.path.dirname(_HERE), 'include')
+    return [SOURCE] + [os.path.join(include, f) for f in ('elx_ops.h', 'elx_abi.h')]
+
+
 def stamp() -> str:
-    """What a build carries: the digest of its source and of the header it calls through, and the version of torch."""
+    """What a build carries: the digest of its sources, and the version of torch."""
     h = hashlib.sha256()
-    for path in (SOURCE, os.path.join(os.path.dirname(_HERE), 'include', 'elx_ops.h')):
+    for path in source_files():
         with open(path, 'rb') as f:
             h.update(f.read())
     return f'{h.hexdigest()[:16]} torch {torch.__version__}'
