@@ -57,8 +57,18 @@ def build(verbose: bool = True) -> str:
             print(out)
     if failed:
         raise RuntimeError('\n'.join(failed))
-    build_torch_ext(verbose)
+    if torch_ext_buildable():
+        build_torch_ext(verbose)
+    else:    # the step with 32-bit moments does without; what needs it raises
+        print('_elx_torch.so is not built: it takes g++ and the headers of torch.  layer_norm, embedding and reading 8-bit moments '
+              'will raise.', file=sys.stderr, flush=True)
     return OUTPUT
+
+
+def torch_ext_buildable() -> bool:
+    """Whether the host compiler and the headers that the Python extension takes are here."""
+    import torch
+    return shutil.which('g++') is not None and os.path.isdir(os.path.join(os.path.dirname(torch.__file__), 'include'))
 
 
 def build_torch_ext(verbose: bool = True) -> str:
@@ -100,7 +110,7 @@ def is_stale() -> bool:
     """A built library is missing, or was built from other sources than the ones beside it."""
     return (not os.path.exists(OUTPUT) or built_source_sha(OUTPUT) != source_sha16() or not os.path.exists(OPS_OUTPUT)
             or _ops_abi.built_source_sha(OPS_OUTPUT) != _ops_abi.source_sha16()
-            or _torch_ext.built_stamp(_torch_ext.LIB_PATH) != _torch_ext.stamp())
+            or (_torch_ext.built_stamp(_torch_ext.LIB_PATH) != _torch_ext.stamp() and torch_ext_buildable()))
 
 
 def ensure_built(verbose: bool = False) -> str:

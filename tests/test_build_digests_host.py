@@ -1,4 +1,5 @@
-"""Every header of this repository that a built file includes is part of the digest it carries: an edit makes the build stale."""
+"""Builds: every header of this repository that a built file includes is part of the digest it carries, so that an edit makes the
+build stale; without a host compiler the libraries of the step are built all the same."""
 import os
 import re
 
@@ -39,3 +40,30 @@ def test_an_edited_header_makes_the_extension_stale(monkeypatch, tmp_path):
         copy.write_bytes(open(name, 'rb').read() + b'\n')
         monkeypatch.setattr(_torch_ext, 'source_files', lambda i=i, copy=str(copy): files[:i] + [copy] + files[i + 1:])
         assert B.is_stale()
+
+
+def test_the_libraries_are_built_without_a_host_compiler(monkeypatch, capsys):
+    """The step with 32-bit moments needs hipcc alone, as before there was an extension."""
+    ran = []
+
+    class Done:
+        returncode = 0
+
+        def __init__(self, cmd, **kw):
+            ran.append(cmd[0])
+
+        def communicate(self):
+            return '', None
+
+    monkeypatch.setattr(B.subprocess, 'Popen', Done)
+    monkeypatch.setattr(B.subprocess, 'run', lambda cmd, **kw: ran.append(cmd[0]))
+    which = B.shutil.which
+    monkeypatch.setattr(B.shutil, 'which', lambda name: None if name == 'g++' else which(name))
+    assert B.build(verbose=False) == B.OUTPUT
+    assert len(ran) == 2 and 'g++' not in ran and 'layer_norm' in capsys.readouterr().err
+    # nothing that could be built is stale; loading the extension is refused by itself
+    monkeypatch.setattr(_torch_ext, 'stamp', lambda: 'other')
+    assert not B.is_stale()
+    monkeypatch.setattr(_torch_ext, '_ext', None)
+    with pytest.raises(RuntimeError, match='missing or was built from something else'):
+        _torch_ext.load()
