@@ -561,8 +561,8 @@ struct shape {    // accesses per lane, wavefronts per row, lanes per row of a w
     static constexpr int accesses = N, waves = W, lanes = L;
 };
 
-// wavefronts per row and accesses per lane, the latter rounded up to what is compiled
-template <int V, typename F>
+// wavefronts per row and accesses per lane, the latter rounded up to what is compiled; FEW: fewer than 4096 rows
+template <int V, bool FEW, typename F>
 int dispatch_rows(uint64_t rows, uint32_t cols, F &&launch) {
     const uint32_t accesses = (cols + kWave * V - 1) / (kWave * V);    // wavefront-wide accesses of a row
     // Four wavefronts read a long row in a quarter of the steps, one wavefront needs no barrier:
@@ -570,7 +570,7 @@ int dispatch_rows(uint64_t rows, uint32_t cols, F &&launch) {
     //   32768 x 4096 bf16   79              100                8192 x 2048 bf16   14              10.6
     //    8191 x 1025 fp16   18               25                8191 x 1023 fp16   13.9            12.6
     // With few rows it is the steps that count (1024 x 2048 bf16: 4.5 us with four, 5.5 with one; 4096 x 2048: 7.1, 6.8).
-    if (accesses >= (V == 1 ? 17 : 8) || (rows < 4096 && accesses >= 4)) {
+    if (accesses >= (V == 1 ? 17 : 8) || ((FEW || rows < 4096) && accesses >= 4)) {
         const uint32_t n = (accesses + 3) / 4;
         if (n <= 1) return launch(shape<1, 4>());
         if (n <= 2) return launch(shape<2, 4>());
@@ -591,15 +591,17 @@ int dispatch_rows(uint64_t rows, uint32_t cols, F &&launch) {
     if (accesses <= 1) return launch(shape<1, 1>());
     if (accesses <= 2) return launch(shape<2, 1>());
     if (accesses <= 4) return launch(shape<4, 1>());
-    if (accesses <= 8) return launch(shape<8, 1>());
-    if constexpr (V == 1)
-        if (accesses <= 16) return launch(shape<16, 1>());
+    if constexpr (!FEW) {
+        if (accesses <= 8) return launch(shape<8, 1>());
+        if constexpr (V == 1)
+            if (accesses <= 16) return launch(shape<16, 1>());
+    }
     return ELX_E_SIZE;
 }
 
 template <int D, int V>
 int dispatch_fwd(const Fwd &a) {
-    return dispatch_rows<V>(a.rows, a.cols, [&](auto s) { return launch_fwd<D, V, s.accesses, s.waves, s.lanes>(a); });
+    return dispatch_rows<V, false>(a.rows, a.cols, [&](auto s) { return launch_fwd<D, V, s.accesses, s.waves, s.lanes>(a); });
 }
 
 struct Bwd {
@@ -643,6 +645,7 @@ int launch_bwd(const Bwd &a) {
 // 4096 17 against 15.7), with 64 or 128 bytes of a row per workgroup of the sums: the narrower, the more workgroups, the wider,
 // the better the reads (1024 x 2048 bf16 6.9 us with 64 and 9.4 with 128, 1024 x 11008 bf16 26 and 20).
 constexpr uint64_t kFewRows = 1024;
+static_assert(kFewRows < 4096, "FEW of dispatch_rows");
 constexpr uint32_t kNarrowBytes = 6144;    // of a row
 
 template <int D, int V, int N, int W, int L>
@@ -662,15 +665,16 @@ int launch_few(const Bwd &a) {
 template <int D, int V>
 int dispatch_bwd(const Bwd &a) {
     if (a.rows <= kFewRows)
-        return dispatch_rows<V>(a.rows, a.cols, [&](auto s) { return launch_few<D, V, s.accesses, s.waves, s.lanes>(a); });
+        return dispatch_rows<V, true>(a.rows, a.cols, [&](auto s) { return launch_few<D, V, s.accesses, s.waves, s.lanes>(a); });
     if (a.cols <= 4 * V) return launch_bwd<D, V, 1, 1, 4>(a);
     if (a.cols <= 8 * V) return launch_bwd<D, V, 1, 1, 8>(a);
     if (a.cols <= 16 * V) return launch_bwd<D, V, 1, 1, 16>(a);
     if (a.cols <= 32 * V) return launch_bwd<D, V, 1, 1, 32>(a);
     const uint32_t waves = bwd_waves(a.cols);
     const uint32_t n = (a.cols + waves * kWave * V - 1) / (waves * kWave * V);
+    // more than one wavefront: cols > 256 waves, which is more than 4 elements per lane
 #define ELX_CASE(WAVES, ACCESSES)                                                  \
-    if constexpr (ACCESSES * V <= (WAVES == 16 ? 16 : 8))                           \
+    if constexpr (ACCESSES * V <= (WAVES == 16 ? 16 : 8) && (WAVES == 1 || ACCESSES * V > 4)) \
         if (waves == WAVES && n <= ACCESSES) return launch_bwd<D, V, ACCESSES, WAVES>(a);
     ELX_CASE(1, 1)
     ELX_CASE(1, 2)
