@@ -193,7 +193,25 @@ __device__ __forceinline__ void forget(T &x) {
         u32x4 y = __builtin_bit_cast(u32x4, x);
         asm volatile("" : "+v"(y));
         x = __builtin_bit_cast(T, y);
+    } else {    // one element
+        asm volatile("" : "+v"(x));
     }
+}
+
+// One element of a row as a buffer of its own, at a byte offset: behind its end a load gives zero and a store does nothing.
+template <int D>
+__device__ __forceinline__ typename Elem<D>::scalar row_load(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+    if constexpr (D == ELX_F32)
+        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, (int)at, 0, 0));
+    else
+        return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, (int)at, 0, 0);
+}
+template <int D>
+__device__ __forceinline__ void row_store(__amdgpu_buffer_rsrc_t r, uint32_t at, typename Elem<D>::scalar x) {
+    if constexpr (D == ELX_F32)
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), r, (int)at, 0, 2);    // non-temporal
+    else
+        __builtin_amdgcn_raw_buffer_store_b16(x, r, (int)at, 0, 2);
 }
 
 constexpr int kBwdWaves = 16;
@@ -212,9 +230,21 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
     typedef typename Pack<D, V>::type pack_t;
     constexpr int kGroups = kBwdWaves / W * (kWave / L);    // rows in flight
     constexpr bool kAhead = V * N <= 8;    // a lane has 128 registers: no room for a second row beyond that
+    // 16 elements one by one: with a 64-bit address and a mask for each access, and w held, registers spilled to memory (2000 x
+    // 16383 fp32 695 us, bf16 127; 91 and 56 without).  The row is a buffer and an access one offset into it; the workgroup has one
+    // row, so the buffer is the same in all lanes.
+    constexpr bool kBuffer = V == 1 && N > 8;
+    static_assert(!kBuffer || W == kBwdWaves, "a row per workgroup");
+    // h and t are computed once more for dx where the registers to keep them are short; 8 elements of 16 wavefronts keep them
+    // (8191 x 4097 bf16 107 us, 111 with them computed again; 2047 x 769 fp16, two wavefronts, 8.0 and 6.8).
+    constexpr bool kOnceMore = V > 1 || kBuffer || W < kBwdWaves;
+    const uint32_t row_bytes = cols * (uint32_t)sizeof(typename Elem<D>::scalar);
+    constexpr int kUnrollSums = kBuffer ? 4 : W;
     __shared__ float part[2][2][W > 1 ? kGroups : 1][W];
     const int wave = threadIdx.x / kWave % W, lane = threadIdx.x % L;
-    const int group = threadIdx.x / kWave / W * (kWave / L) + threadIdx.x % kWave / L;
+    const int group = W == kBwdWaves ? 0 : threadIdx.x / kWave / W * (kWave / L) + threadIdx.x % kWave / L;
+    const uint32_t first = ((uint32_t)wave * L + lane) * (uint32_t)sizeof(pack_t);    // byte offset of this lane's first access
+    auto offset_of = [&](int n) { return first + (uint32_t)n * (W * L * (uint32_t)sizeof(pack_t)); };
     float dw[N][V], db[N][V];
     pack_t pw[N];
 #pragma unroll
@@ -226,7 +256,7 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
             dw[n][k] = db[n][k] = 0.0f;
             one[k] = 1.0f;
         }
-        pw[n] = w && c < cols ? *reinterpret_cast<const pack_t *>(w + c) : pack<D, V>(one);
+        if constexpr (!kBuffer) pw[n] = w && c < cols ? *reinterpret_cast<const pack_t *>(w + c) : pack<D, V>(one);
     }
     const float inv = 1.0f / (float)cols;
     // every wavefront takes the same number of turns: the barriers inside are the workgroup's
@@ -239,9 +269,16 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
         const bool live = row < rows;
         m = live ? mean_in[row] : 0.0f;
         r = live ? rstd_in[row] : 0.0f;
+        const __amdgpu_buffer_rsrc_t rx = tile_rsrc(kBuffer && live ? x + row * x_stride : x, kBuffer && live ? row_bytes : 0);
+        const __amdgpu_buffer_rsrc_t rg = tile_rsrc(kBuffer && live ? dy + row * dy_stride : dy, kBuffer && live ? row_bytes : 0);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const uint32_t c = ((uint32_t)(n * W + wave) * L + lane) * V;
+            if constexpr (kBuffer) {
+                qx[n] = row_load<D>(rx, offset_of(n));
+                qg[n] = row_load<D>(rg, offset_of(n));
+                continue;
+            }
             qx[n] = pack_t{};
             qg[n] = pack_t{};
             if (live && c < cols) {
@@ -255,6 +292,15 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
                     qg[n] = *from;
                 }
             }
+        }
+    };
+    const __amdgpu_buffer_rsrc_t rw = tile_rsrc(kBuffer && w ? w : x, kBuffer && w ? row_bytes : 0);
+    auto weight_of = [&](int n, float (&wt)[V]) {
+        if constexpr (kBuffer) {    // from the cache, twice: there is no room for it either
+            const float got = Elem<D>::to_f32(row_load<D>(rw, offset_of(n)));
+            wt[0] = w ? got : 1.0f;
+        } else {
+            unpack<D, V>(pw[n], wt);
         }
     };
     fetch(0, px, pg, mean, rstd);
@@ -278,10 +324,10 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
             float h[V], g[V], wt[V];
             unpack<D, V>(px[n], h);
             unpack<D, V>(pg[n], g);
-            unpack<D, V>(pw[n], wt);
+            weight_of(n, wt);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                h[k] = c < cols ? (h[k] - mean) * rstd : 0.0f;
+                h[k] = kBuffer || c < cols ? (h[k] - mean) * rstd : 0.0f;
                 dw[n][k] = fmaf(g[k], h[k], dw[n][k]);
                 db[n][k] += g[k];
                 const float t = g[k] * wt[k];
@@ -300,7 +346,7 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
             }
             __syncthreads();
             st = sth = 0.0f;
-#pragma unroll
+#pragma unroll kUnrollSums
             for (int i = 0; i < W; ++i) {
                 st += p[i];
                 sth += q[i];
@@ -309,20 +355,26 @@ __global__ __launch_bounds__(kBwdThreads) void layer_norm_bwd_kernel(
         st *= inv;
         sth *= inv;
         if (row < rows && dx) {    // h and t once more, from the row as it came: cheaper than the registers to keep them
+            const __amdgpu_buffer_rsrc_t rd = tile_rsrc(kBuffer ? dx + row * cols : dx, kBuffer ? row_bytes : 0);
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                forget(px[n]);
-                forget(pg[n]);
-                forget(pw[n]);
+                if constexpr (kOnceMore) {
+                    forget(px[n]);
+                    forget(pg[n]);
+                    if constexpr (!kBuffer) forget(pw[n]);
+                }
                 const uint32_t c = ((uint32_t)(n * W + wave) * L + lane) * V;
-                if (c < cols) {
+                if (kBuffer || c < cols) {
                     float h[V], g[V], wt[V], o[V];
                     unpack<D, V>(px[n], h);
                     unpack<D, V>(pg[n], g);
-                    unpack<D, V>(pw[n], wt);
+                    weight_of(n, wt);
 #pragma unroll
                     for (int k = 0; k < V; ++k) o[k] = (g[k] * wt[k] - st - (h[k] - mean) * rstd * sth) * rstd;
-                    __builtin_nontemporal_store(pack<D, V>(o), reinterpret_cast<pack_t *>(dx + row * cols + c));
+                    if constexpr (kBuffer)
+                        row_store<D>(rd, offset_of(n), pack<D, V>(o));
+                    else
+                        __builtin_nontemporal_store(pack<D, V>(o), reinterpret_cast<pack_t *>(dx + row * cols + c));
                 }
             }
         }
