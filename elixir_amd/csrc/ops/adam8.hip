@@ -11,9 +11,11 @@
 // (elx_kernels.hip): one tile per workgroup, tiles in address order, the number of resident workgroups held by an LDS
 // reservation that no thread touches.
 //
-// Bound by HBM: 1.315e9 elements (OPT-1.3B in bf16) take 3.17 ms = 6.6 TB/s, the rate of a copy, against 5.53 ms with the 32-bit
-// state; 16 Mi fp32 elements whose data stay in the memory-side cache 39 us against 66.  Reading the values of 134 Mi elements
-// takes 187 us to fp32 (7.2 TB/s) and 117 us to bf16.
+// Bound by HBM: 1.31e9 elements (OPT-1.3B in bf16) take 3.17 to 3.19 ms = 6.6 TB/s, the rate of a copy, against 5.53 ms with the
+// 32-bit state; 5.4e8 elements with fp32 gradients (20 bytes each) 1.69 ms = 6.4 TB/s against 2.57; 16 Mi fp32 elements whose data
+// stay in the memory-side cache 39 us against 66.  Reading the values of 128 Mi elements takes 187 us to fp32 (7.2 TB/s) and 115 us
+// to bf16 (7.0 TB/s) where the codes were read before, 134 us behind a step (6.0 TB/s).  Writing as many from fp32 takes 143 us a
+// moment (4.7 TB/s): checkpoints are loaded with it, a step does not.
 //
 // Arithmetic: fp32; unscale and moments have the bits of the 32-bit update (fused multiply-adds written as fmaf,
 // -ffp-contract=off), the change of the master weight is that update's to within 2^-20.  Only the new moments are rounded to
@@ -36,7 +38,8 @@ constexpr int kVec = 4;
 static_assert(kTile == elx_host::kTile, "a tile of the update tables is a block of the 8-bit code");
 
 // Resident workgroups per compute unit when the caller names no number.  1.3e9 elements in bf16: 3.40 ms with 16, 3.25 with 20,
-// 3.29 with 24, 3.47 with 32; where the gradient is divided by a scale that is no power of two 3.30 with 20, 3.27 with 24.
+// 3.29 with 24, 3.47 with 32; where the gradient is divided by a scale that is no power of two 3.30 with 20, 3.27 with 24: what is
+// taken lies between.  5.4e8 elements in bf16: 1.31 ms with 18, 1.30 with 20, 22 and 24.
 constexpr uint32_t kBlocksPerCu = 22;
 
 // cache policy, as in the 32-bit update: everything streams; the low-precision copy stays in the memory-side cache; all does
