@@ -41,7 +41,7 @@ import torch
 from torch.nn import Parameter
 
 from . import _abi, _ops_abi
-from .chunk import (Chunk, DeviceTable, StatsArena, dtype_code, gpu_device, keep_grads_cached, kernel_device, launch_grad_stats,
+from .chunk import (Chunk, DeviceTable, StatsArena, dtype_code, keep_grads_cached, kernel_device, launch_grad_stats,
                     read_grad_stats, resolve_pending_stats, stats_launch_blocks)
 from .grad_scaler import BaseGradScaler, ConstantGradScaler, DynamicGradScaler
 from .hybrid_adam import CPUAdam, FusedAdam, HybridAdam
@@ -258,8 +258,8 @@ class ElixirOptimizer(torch.optim.Optimizer):
         pooled = getattr(module, 'pooled_elems', 0)
         if pooled:    # the moments in one allocation: 8 bytes per element, or two codes and two exponents per block
             state8 = getattr(optimizer, 'state_bits', 32) == 8
-            reserve_device_pool(2 * pooled + 2 * -(-pooled // _ops_abi.STATE_BLOCK) if state8 else 8 * pooled, gpu_device(), minimum=0,
-                                slack=2 << 20)
+            reserve_device_pool(2 * pooled + 2 * -(-pooled // _ops_abi.STATE_BLOCK) if state8 else 8 * pooled,
+                                next(t.device for t in shards if t.is_cuda), minimum=0, slack=2 << 20)
         self._stats_table = None
         self._all_stats_table = None
         self._stats_workspace: Dict = {}
