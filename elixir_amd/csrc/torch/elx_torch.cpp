@@ -140,7 +140,9 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const bool want_w = (affine & 1) && ctx->needs_input_grad(edge++);
         const bool want_b = (affine & 2) && ctx->needs_input_grad(edge++);
         Tensor dx, dw, db;
-        if (at::GradMode::is_enabled()) {    // the gradient is to be differentiated: torch's operators
+        if (at::GradMode::is_enabled() || !grad.has_storage()) {    // to be differentiated, or many at once: torch's operators
+            const bool create_graph = at::GradMode::is_enabled();
+            const at::AutoGradMode record(true);
             // With respect to aliases: the saved tensors carry their history, and where one of them is an ancestor of the
             // other (one norm in two layers) the derivative would run on through it, a path that is the outer pass's.
             const Tensor a = x.view_as(x), w = weight.defined() ? weight.view_as(weight) : weight;
@@ -150,7 +152,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
             if (want_w) leaves.push_back(w);
             if (want_b) leaves.push_back(b);
             const Tensor y = at::layer_norm(a, shape, w, b, ctx->saved_data["eps"].toDouble());
-            auto got = torch::autograd::grad({y}, leaves, {grad}, std::nullopt, true);
+            auto got = torch::autograd::grad({y}, leaves, {grad}, std::nullopt, create_graph);
             size_t i = 0;
             if (want_x) dx = got[i++];
             if (want_w) dw = got[i++];
@@ -241,12 +243,14 @@ struct Embedding : torch::autograd::Function<Embedding> {
         const c10::DeviceGuard guard(grad.device());
         TORCH_CHECK(cols == 0 || index.numel() == grad.numel() / cols, "embedding: a saved tensor came back in another shape");
         check_saved("embedding", index, ctx->saved_data["wide"].toBool() ? at::kLong : at::kInt, grad.device(), index.numel());
-        if (at::GradMode::is_enabled()) {    // the gradient is to be differentiated: torch's operators
+        if (at::GradMode::is_enabled() || !grad.has_storage()) {    // to be differentiated, or many at once: torch's operators
+            const bool create_graph = at::GradMode::is_enabled();
+            const at::AutoGradMode record(true);
             const Tensor inside = index.ge(0).logical_and(index.lt(rows));
             const Tensor table = at::zeros({rows, cols}, options).requires_grad_();
             const Tensor y = at::embedding(table, index.where(inside, at::zeros_like(index)), padding);
             const Tensor dy = (grad * scale).masked_fill(inside.logical_not().unsqueeze(-1), 0);
-            return {Tensor(), torch::autograd::grad({y}, {table}, {dy}, std::nullopt, true)[0], Tensor(), Tensor()};
+            return {Tensor(), torch::autograd::grad({y}, {table}, {dy}, std::nullopt, create_graph)[0], Tensor(), Tensor()};
         }
         Tensor dtable = at::empty({rows, cols}, options);
         const int64_t n = index.numel();

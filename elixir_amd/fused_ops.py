@@ -6,7 +6,7 @@ The reference swaps ``F.layer_norm`` for a third party's fused kernel (elixir/ke
 embedding to torch.  Both functions take device tensors in fp32, fp16 or bf16, compute in fp32 and round once, run on the
 current stream of the tensors' device, allocate what they return (and, in backward, a workspace) through torch's allocator,
 synchronise nothing, and can be captured into a graph.  A gradient that is itself to be differentiated
-(``create_graph=True``) is computed by torch's own operators; forward-mode derivatives and tracing are refused.  What the
+(``create_graph=True``) and gradients for many at once (``is_grads_batched=True``) are computed by torch's own operators; forward-mode derivatives and tracing are refused.  What the
 functions cannot take they refuse; the modules fall back to torch instead, so that a model keeps running wherever it ran."""
 from typing import Optional, Sequence, Union
 
